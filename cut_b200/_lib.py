@@ -10,10 +10,10 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libcutb.so")
 
-OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT, ERR_RANGE = range(7)
+OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT, ERR_RANGE, ERR_PAGES = range(8)
 Q8_0, Q4_0, Q4_K, Q5_K, Q6_K, BF16, Q4_1, Q5_0 = 0, 1, 2, 3, 4, 5, 6, 7  # from Q5_K on: cutb_dequant only
 F32, F16 = 0, 1
-UNARY_RELU_SQUARE, NO_TOKEN = 200, 0xFFFFFFFF
+UNARY_RELU_SQUARE, NO_TOKEN, NO_PAGE = 200, 0xFFFFFFFF, 0xFFFFFFFF
 GLU_NONE, GLU_CLAMPED = 0, 1
 DENSE_AUTO, DENSE_MATVEC, DENSE_TC, DENSE_SIMT = -1, 0, 1, 2
 ROT_HALVES, ROT_NEIGHBOURS = 0, 1
@@ -42,6 +42,9 @@ EXPORTS = [
     "cutb_latent_kv_write", "cutb_latent_attention", "cutb_latent_takes_split_queries", "cutb_latent_splits", "cutb_latent_workspace_bytes", "cutb_latent_values",
     "cutb_latent_prefill_supported", "cutb_latent_prefill", "cutb_moe_route", "cutb_moe_scatter", "cutb_moe_matmul", "cutb_expert_up",
     "cutb_expert_down",
+    "cutb_paged_layer_bytes", "cutb_paged_kv_write", "cutb_paged_kv_read", "cutb_paged_workspace_bytes", "cutb_paged_attention",
+    "cutb_pages_workspace_bytes", "cutb_pages_reserve", "cutb_pages_fork", "cutb_pages_free", "cutb_pages_compact", "cutb_pages_copy",
+    "cutb_sample",
 ]
 
 
@@ -171,6 +174,40 @@ class ExpertDesc(C.Structure):
     ]
 
 
+class PagedDesc(C.Structure):
+    _fields_ = [
+        ("pages", C.c_void_p), ("page_bytes", C.c_uint64), ("ld_table", C.c_uint64),
+        ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+        ("tables", C.c_void_p), ("lengths", C.c_void_p), ("slots", C.c_void_p), ("starts", C.c_void_p),
+        ("n_slots", C.c_uint32), ("n_seqs", C.c_uint32), ("n_tokens", C.c_uint32), ("max_new", C.c_uint32),
+        ("dtype", C.c_int32), ("n_heads", C.c_uint32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("ldq", C.c_uint64), ("ldk", C.c_uint64), ("ldv", C.c_uint64),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("ldq_out", C.c_uint64), ("ldk_out", C.c_uint64), ("ldv_out", C.c_uint64),
+        ("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("rot_dims", C.c_uint32), ("max_pos", C.c_uint32), ("rot_pairing", C.c_int32),
+        ("scale", C.c_float), ("window", C.c_uint32), ("out", C.c_void_p), ("ldo", C.c_uint64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("status", C.c_void_p),
+    ]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [
+        ("pages", C.c_void_p), ("page_bytes", C.c_uint64), ("ld_table", C.c_uint64),
+        ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("n_slots", C.c_uint32), ("n", C.c_uint32),
+        ("tables", C.c_void_p), ("lengths", C.c_void_p), ("refs", C.c_void_p),
+        ("items", C.c_void_p), ("others", C.c_void_p), ("counts", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("status", C.c_void_p),
+    ]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("ld", C.c_uint64), ("rows", C.c_uint32), ("vocab", C.c_uint32), ("dtype", C.c_int32),
+        ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("u", C.c_void_p),
+        ("tokens", C.c_void_p), ("logprobs", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
 MAX_PEERS = 8
 
 
@@ -214,7 +251,7 @@ def _bind_layers(l: C.CDLL) -> None:
                        ("cutb_window_attention_decode", WindowAttnDesc), ("cutb_latent_kv_write", LatentAttnDesc),
                        ("cutb_latent_attention", LatentAttnDesc), ("cutb_latent_values", LatentAttnDesc), ("cutb_latent_prefill", LatentAttnDesc),
                        ("cutb_moe_route", MoeDesc), ("cutb_moe_scatter", MoeDesc), ("cutb_moe_matmul", MoeDesc), ("cutb_expert_up", ExpertDesc),
-                       ("cutb_expert_down", ExpertDesc)):
+                       ("cutb_expert_down", ExpertDesc), ("cutb_sample", SampleDesc)):
         getattr(l, name).restype = C.c_int
         getattr(l, name).argtypes = [C.POINTER(desc), C.c_void_p]
     for name, kind in (("cutb_latent_splits", C.c_uint32), ("cutb_latent_workspace_bytes", C.c_uint64), ("cutb_latent_prefill_supported", C.c_int),
@@ -232,6 +269,16 @@ def _bind_layers(l: C.CDLL) -> None:
 
 
 def _bind_quantized(l: C.CDLL) -> None:
+    for name, desc in (("cutb_paged_kv_write", PagedDesc), ("cutb_paged_kv_read", PagedDesc), ("cutb_paged_attention", PagedDesc),
+                       ("cutb_pages_reserve", PagesDesc), ("cutb_pages_fork", PagesDesc), ("cutb_pages_free", PagesDesc),
+                       ("cutb_pages_compact", PagesDesc), ("cutb_pages_copy", PagesDesc)):
+        getattr(l, name).restype = C.c_int
+        getattr(l, name).argtypes = [C.POINTER(desc), C.c_void_p]
+    for name, desc in (("cutb_paged_workspace_bytes", PagedDesc), ("cutb_pages_workspace_bytes", PagesDesc)):
+        getattr(l, name).restype = C.c_uint64
+        getattr(l, name).argtypes = [C.POINTER(desc)]
+    l.cutb_paged_layer_bytes.restype = C.c_uint64
+    l.cutb_paged_layer_bytes.argtypes = [C.c_uint32] * 3
     l.cutb_qmatmul_workspace_bytes.restype = C.c_uint64
     l.cutb_qmatmul_workspace_bytes.argtypes = [C.POINTER(QMatmulDesc)]
     l.cutb_qmatmul_select_variant.restype = C.c_int

@@ -185,6 +185,7 @@ const char *cutb_status_string(int status) {
     case CUTB_ERR_WORKSPACE: return "workspace missing or too small";
     case CUTB_ERR_TIMEOUT: return "device-side wait timed out";
     case CUTB_ERR_RANGE: return "activation outside the fp16 operand range";
+    case CUTB_ERR_PAGES: return "too few free pages";
     default: return "unknown status";
   }
 }

@@ -147,6 +147,18 @@ int window_kv_write_launch(const cutb_window_attn_desc &d, cudaStream_t stream);
 int window_attention_launch(const cutb_window_attn_desc &d, cudaStream_t stream);
 int window_attention_decode_launch(const cutb_window_attn_desc &d, cudaStream_t stream);
 
+// A cache in pages of 4-bit elements (paged_cache.cu, paged_attention.cu), sampling (sample.cu).
+int paged_kv_write_launch(const cutb_paged_desc &d, cudaStream_t stream);
+int paged_kv_read_launch(const cutb_paged_desc &d, cudaStream_t stream);
+uint64_t paged_attention_workspace(const cutb_paged_desc &d);
+int paged_attention_launch(const cutb_paged_desc &d, cudaStream_t stream);
+int pages_reserve_launch(const cutb_pages_desc &d, cudaStream_t stream);
+int pages_fork_launch(const cutb_pages_desc &d, cudaStream_t stream);
+int pages_free_launch(const cutb_pages_desc &d, cudaStream_t stream);
+int pages_compact_launch(const cutb_pages_desc &d, cudaStream_t stream);
+int pages_copy_launch(const cutb_pages_desc &d, cudaStream_t stream);
+int sample_launch(const cutb_sample_desc &d, cudaStream_t stream);
+
 // Load-time repacks (repack.cu), bit-exact with the reference's CPU loader / runner code.
 int separate_launch(int format, const void *raw, void *values, void *scales, uint64_t rows, uint64_t cols, cudaStream_t stream);
 int transpose_launch(uint32_t elem_bytes, const void *in, void *out, uint32_t R, uint32_t C, uint64_t ldi, uint64_t ldo,

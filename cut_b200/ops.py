@@ -513,6 +513,155 @@ def expert_desc(experts: int, top: int, width: int, ff: int, W: torch.Tensor, id
     return d
 
 
+# ---- a cache in pages of 4-bit elements (paged.PagedCache) -----------------------------------------------------------------
+_ELEMENTS = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+
+
+def _here(what: str, *tensors) -> None:
+    """The pointers of a call belong to the current device."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.get_device() == torch.cuda.current_device()):
+            raise RuntimeError(f"{what}: every tensor is on the current CUDA device")
+
+
+def _rows(t: torch.Tensor, heads: int, head_dim: int, what: str) -> torch.Tensor:
+    if t.dtype not in _ELEMENTS or t.dim() != 2 or t.shape[1] != heads * head_dim or (t.numel() and t.stride(1) != 1):
+        raise RuntimeError(f"{what}: rows of {heads} x {head_dim} elements in float32, float16 or bfloat16, with unit stride")
+    return t
+
+
+def _int_vector(t: torch.Tensor | None, n: int | None, what: str):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1) or (n is not None and t.numel() != n):
+        raise RuntimeError(f"{what}: an int32 vector on the device" + (f" of {n} entries" if n is not None else ""))
+    return t.data_ptr()
+
+
+def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=None, max_new: int | None = None, layer: int = 0, status=None):
+    """cutb_paged_desc of a call over `cache` (paged.PagedCache): sequence i is slot slots[i] (None: slot i), its rows are starts[i] ..
+    starts[i + 1] - 1 of n_tokens (None: row i).  max_new: at most so many rows of a sequence (None: as many as there are)."""
+    _here("paged", cache.pages, cache.tables, cache.lengths, starts, slots, status)
+    d = L.PagedDesc()
+    part = cache.layer_bytes() if layer else 0
+    if layer < 0 or (layer and (layer + 1) * part > cache.pages.shape[1]):
+        raise RuntimeError("paged: no such layer in this cache")
+    d.pages, d.page_bytes, d.ld_table = cache.pages.data_ptr() + layer * part, cache.pages.stride(0), cache.tables.stride(0)
+    d.n_pages, d.page_tokens, d.n_kv_heads, d.head_dim = cache.pages.shape[0], cache.page_tokens, cache.n_kv_heads, cache.head_dim
+    d.tables, d.lengths, d.n_slots = cache.tables.data_ptr(), cache.lengths.data_ptr(), cache.tables.shape[0]
+    d.n_tokens, d.dtype = n_tokens, _ELEMENTS[dtype]
+    d.n_seqs = starts.numel() - 1 if starts is not None else slots.numel() if slots is not None else min(n_tokens, d.n_slots)
+    if d.n_seqs < 0 or (starts is None and n_tokens < d.n_seqs):
+        raise RuntimeError("paged: starts has an entry more than there are sequences; without it every sequence has a row")
+    d.starts, d.slots = _int_vector(starts, None, "starts"), _int_vector(slots, d.n_seqs, "slots")
+    d.max_new = (1 if starts is None else max(1, n_tokens)) if max_new is None else max_new
+    st = status if status is not None else cache.status
+    d.status = st.data_ptr() if st is not None else None
+    return d
+
+
+def paged_kv_write(cache, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None, starts=None,
+                   slots=None, max_new: int | None = None, cos_t=None, sin_t=None, rot_dims: int = 0, pairing: int = L.ROT_HALVES, layer: int = 0,
+                   status=None):
+    """Stores the rows k, v [n, n_kv_heads * head_dim] of the sequences' last tokens (cache.lengths counts them already), keys turned at
+    their positions, in 4 bits; with q [n, n_heads * head_dim] returns the turned queries."""
+    hk, hd = cache.n_kv_heads, cache.head_dim
+    _rows(k, hk, hd, "paged_kv_write: k"), _rows(v, hk, hd, "paged_kv_write: v")
+    if v.dtype != k.dtype or v.shape[0] != k.shape[0] or (q is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0])):
+        raise RuntimeError("paged_kv_write: q, k and v have one type and one number of rows")
+    if rot_dims and (cos_t is None or sin_t is None or cos_t.shape != sin_t.shape or cos_t.dim() != 2 or cos_t.shape[1] * 2 != rot_dims or
+                     any(t.dtype != torch.float32 or not t.is_contiguous() for t in (cos_t, sin_t))):
+        raise RuntimeError("paged_kv_write: float32 tables [positions, rot_dims / 2]")
+    _here("paged_kv_write", k, v, q, q_out, cos_t, sin_t)
+    d = paged_desc(cache, k.shape[0], k.dtype, starts=starts, slots=slots, max_new=max_new, layer=layer, status=status)
+    d.k, d.ldk, d.v, d.ldv = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
+    if q is not None:
+        heads = q.shape[1] // hd
+        _rows(q, heads, hd, "paged_kv_write: q")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif q_out.dtype != q.dtype or q_out.shape != q.shape:
+            raise RuntimeError("paged_kv_write: q_out is like q")
+        _rows(q_out, heads, hd, "paged_kv_write: q_out")
+        d.n_heads, d.q, d.ldq, d.q_out, d.ldq_out = heads, q.data_ptr(), q.stride(0), q_out.data_ptr(), q_out.stride(0)
+    if rot_dims:
+        d.cos_table, d.sin_table, d.max_pos = cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0]
+    d.rot_dims, d.rot_pairing = rot_dims, pairing
+    L.check(L.lib().cutb_paged_kv_write(C.byref(d), _stream_ptr()))
+    return q_out
+
+
+def paged_kv_read(cache, n_tokens: int, *, dtype: torch.dtype = torch.float16, starts=None, slots=None, max_new: int | None = None, layer: int = 0,
+                  status=None):
+    """(keys, values) [n_tokens, n_kv_heads * head_dim] that the sequences' last rows stand for in the cache; rows that no sequence has
+    are zero."""
+    shape = (n_tokens, cache.n_kv_heads * cache.head_dim)
+    new = torch.empty if starts is None else torch.zeros
+    k, v = (new(shape, dtype=dtype, device=cache.pages.device) for _ in range(2))
+    d = paged_desc(cache, n_tokens, dtype, starts=starts, slots=slots, max_new=max_new, layer=layer, status=status)
+    d.k_out, d.ldk_out, d.v_out, d.ldv_out = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
+    L.check(L.lib().cutb_paged_kv_read(C.byref(d), _stream_ptr()))
+    return k, v
+
+
+def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=None, max_new: int | None = None, window: int = 0,
+                    scale: float | None = None, layer: int = 0, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                    status=None) -> torch.Tensor:
+    """Attention of the turned queries q [n, n_heads * head_dim] of the sequences' last tokens over the cache; max_new bounds the rows of
+    a sequence (1 without starts), and a bound near to them lets the call share its work out better."""
+    hd = cache.head_dim
+    _rows(q, n_heads, hd, "paged_attention: q")
+    _here("paged_attention", q, out, workspace)
+    if out is None:
+        out = torch.empty((q.shape[0], n_heads * hd), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise RuntimeError("paged_attention: out is like q")
+    _rows(out, n_heads, hd, "paged_attention: out")
+    d = paged_desc(cache, q.shape[0], q.dtype, starts=starts, slots=slots, max_new=max_new, layer=layer, status=status)
+    d.n_heads, d.q, d.ldq, d.out, d.ldo = n_heads, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0)
+    d.scale, d.window = 1.0 / float(hd) ** 0.5 if scale is None else scale, window
+    need = paged_workspace_bytes(d)
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    L.check(L.lib().cutb_paged_attention(C.byref(d), _stream_ptr()))
+    return out
+
+
+def paged_workspace_bytes(d) -> int:
+    return int(L.lib().cutb_paged_workspace_bytes(C.byref(d)))
+
+
+# ---- the next token ---------------------------------------------------------------------------------------------------
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens: torch.Tensor | None = None,
+           want_logprobs: bool = False, status=None):
+    """int32 [rows]: the next token of each row of logits [rows, vocab] by the random numbers u [rows] in [0, 1); with want_logprobs
+    also the logarithm of its probability.  temperature, top_p, min_p: float32 [rows], top_k: int32 [rows]; None: 1, 1, 0 and no bound.
+    A row without a choice gives -1."""
+    if logits.dim() != 2 or logits.dtype not in _ELEMENTS or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("sample: logits [rows, vocab] in float32, float16 or bfloat16, with unit stride")
+    _here("sample", logits, u, temperature, top_k, top_p, min_p, tokens, status)
+    rows = logits.shape[0]
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    for t, kind in ((u, torch.float32), (temperature, torch.float32), (top_p, torch.float32), (min_p, torch.float32), (top_k, torch.int32),
+                    (tokens, torch.int32)):
+        if t is not None and (t.dtype != kind or t.shape != (rows,) or (rows > 1 and t.stride(0) != 1)):
+            raise RuntimeError("sample: u, temperature, top_p, min_p are float32 and top_k and tokens int32 vectors, a value per row")
+    d = L.SampleDesc()
+    d.logits, d.ld, d.rows, d.vocab, d.dtype = logits.data_ptr(), logits.stride(0), rows, logits.shape[1], _ELEMENTS[logits.dtype]
+    d.temperature, d.top_k, d.top_p, d.min_p, d.u = _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), u.data_ptr()
+    d.tokens, d.status = tokens.data_ptr(), _ptr(status)
+    if not want_logprobs:
+        L.check(L.lib().cutb_sample(C.byref(d), _stream_ptr()))
+        return tokens
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    d.logprobs = logprobs.data_ptr()
+    L.check(L.lib().cutb_sample(C.byref(d), _stream_ptr()))
+    return tokens, logprobs
+
+
 def launch_layer_op(name: str, d) -> None:
     """Launches a layer operator (an entry point that takes a descriptor and a stream)."""
     L.check(getattr(L.lib(), name)(C.byref(d), _stream_ptr()))

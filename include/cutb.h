@@ -42,7 +42,9 @@ enum {
   CUTB_ERR_CUDA = 3,        /* a CUDA runtime call failed (no device, launch error) */
   CUTB_ERR_WORKSPACE = 4,   /* workspace missing or smaller than cutb_qmatmul_workspace_bytes() */
   CUTB_ERR_TIMEOUT = 5,     /* a bounded device-side wait ran out (read from the status word) */
-  CUTB_ERR_RANGE = 6        /* an fp32 activation exceeded the fp16 operand range of the tensor-core GEMM (status word) */
+  CUTB_ERR_RANGE = 6,       /* an fp32 activation exceeded the fp16 operand range of the tensor-core GEMM, or a key or value what the
+                               4-bit cache holds (status word) */
+  CUTB_ERR_PAGES = 7        /* cutb_pages_reserve found too few free pages (status word) */
 };
 
 /* GGUF block formats (interface/loader/gguf/gguf_types.hpp:109-150).  The matmul entry points
@@ -698,6 +700,132 @@ typedef struct cutb_expert_desc {
 } cutb_expert_desc;
 CUTB_API int cutb_expert_up(const cutb_expert_desc *desc, void *stream);
 CUTB_API int cutb_expert_down(const cutb_expert_desc *desc, void *stream);
+
+/*
+ * A cache in pages, four bits per element, for several sequences of lengths of their own (no counterpart in the reference).
+ * A pool holds n_pages pages, page_bytes apart.  A page holds page_tokens consecutive tokens (a power of two, 16 .. 256) of one
+ * sequence: for each layer cutb_paged_layer_bytes() bytes, for each KV head of it page_tokens / 16 units of 16 tokens.  `pages` of
+ * the descriptor is the layer's part of page 0.  Row s of `tables` (ld_table entries) names the pages of sequence slot s in their
+ * order, lengths[s] counts its tokens.
+ *
+ * Quantisation: a group of 32 consecutive elements of a token's head (the last one may be shorter) is held as 4-bit q and a pair of
+ * fp16 numbers, m = fp16(smallest element), d = fp16((largest - m) / 15), q = (x - m) / d rounded to the nearest even and clamped to
+ * 0 .. 15 (0 where d is 0); an element stands for the fp16 number nearest to d q + m.  Elements are held within +-32768, a NaN as
+ * zero; where that changes one, *status becomes CUTB_ERR_RANGE.
+ * A unit, with dp = head_dim rounded up to a multiple of 64 and elements past head_dim zero, has 20 dp bytes:
+ *   keys     bytes 0 .. 8 dp - 1: token t's words of eight elements; element 32 j + 8 b + e is at bit {0, 16, 4, 20, 8, 24, 12, 28}[e]
+ *            of word t dp / 8 + (j / w) 4 w + b w + j % w, w = 4 if dp is a multiple of 128, else 2
+ *   values   bytes 8 dp .. 16 dp - 1: element 16 i + r of token t is in byte {0, 2, 1, 3}[t % 4] of word (i / 4) 128 + ((r % 8) 4 + t / 4) 4
+ *            + i % 4, its low half for r < 8
+ *   scales   then fp16 numbers: of the keys {d, m} of [token][group], of the values {d of four tokens, m of four tokens} of
+ *            [group][t / 4]
+ *
+ * A call works on n_seqs sequences: number i is slot slots[i] (slots null: slot i), and its rows of q, k, v and of the outputs are
+ * starts[i] .. starts[i + 1] - 1 (starts null: row i, one row each), at most max_new of them, n_tokens in all.  They are the last
+ * rows of the sequence: row r has position lengths[slot] - (starts[i + 1] - r).  Rows behind starts[n_seqs] are neither read nor
+ * written.  Element types (dtype) are CUTB_F32, CUTB_F16 or CUTB_BF16.  tables, lengths, slots and starts are device memory, read by the
+ * kernels, so a recorded call serves later steps; n_seqs <= 4096.  A slot past n_slots, rows that do not fit in n_tokens, a length that
+ * is shorter than the new rows or longer than the table, a page that does not exist and a position past max_pos set *status
+ * to CUTB_ERR_INVALID; what they concern is left out (rows and keys as if they were not there), and nothing outside is touched.
+ *
+ *   cutb_paged_kv_write   keys turned at their positions and values into the cache; with q set also q_out = the turned queries.
+ *                         Turned: the first rot_dims elements of a head, tables [max_pos][rot_dims / 2], rot_pairing as in
+ *                         cutb_window_attn_desc; products and sums are rounded separately in fp32.  max_pos is only looked at with
+ *                         rot_dims.  Two rows of a call must not be the same slot's.
+ *   cutb_paged_kv_read    k_out, v_out = the values that the sequences' last rows stand for in the cache
+ *   cutb_paged_attention  out = attention of the (turned) queries: a row at position p sees the keys j <= p with p - j < window
+ *                         (window 0: all of them); a row that sees none gives zeros.  Query head h reads KV head h / (n_heads /
+ *                         n_kv_heads).  Softmax and sums in fp32; fp32 queries and their weights enter the tensor cores as two fp16 terms,
+ *                         16-bit ones as one.  `workspace`: cutb_paged_workspace_bytes(), 256-byte aligned, of no content before or after.
+ *                         Calls that overlap need workspaces of their own.
+ */
+enum { CUTB_NO_PAGE = 0xFFFFFFFFu }; /* an entry of a table behind a sequence's pages */
+typedef struct cutb_paged_desc {
+  void *pages;
+  uint64_t page_bytes, ld_table;
+  uint32_t n_pages, page_tokens, n_kv_heads, head_dim;
+  const uint32_t *tables, *lengths, *slots, *starts;
+  uint32_t n_slots, n_seqs, n_tokens, max_new;
+  int32_t dtype;
+  uint32_t n_heads;
+  const void *q, *k, *v; /* rows of ldq, ldk, ldv elements */
+  uint64_t ldq, ldk, ldv;
+  void *q_out, *k_out, *v_out;
+  uint64_t ldq_out, ldk_out, ldv_out;
+  const float *cos_table, *sin_table;
+  uint32_t rot_dims, max_pos;
+  int32_t rot_pairing;
+  float scale;
+  uint32_t window;
+  void *out;
+  uint64_t ldo;
+  void *workspace;
+  uint64_t workspace_bytes;
+  int *status;
+} cutb_paged_desc;
+CUTB_API uint64_t cutb_paged_layer_bytes(uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_tokens);
+CUTB_API int cutb_paged_kv_write(const cutb_paged_desc *desc, void *stream);
+CUTB_API int cutb_paged_kv_read(const cutb_paged_desc *desc, void *stream);
+CUTB_API uint64_t cutb_paged_workspace_bytes(const cutb_paged_desc *desc);
+CUTB_API int cutb_paged_attention(const cutb_paged_desc *desc, void *stream);
+
+/*
+ * The pages' bookkeeping, on the device: refs[p] counts the slots that hold page p (0: free).  The pool's pages move as whole
+ * pages of page_bytes bytes (a multiple of 16; `pages` is page 0), all layers at once.  items, others and counts (n entries, at
+ * most 1024; copies: 65535) are device memory.  An entry that cannot be served is left out with *status = CUTB_ERR_INVALID.
+ *   cutb_pages_reserve  slot items[i] grows by counts[i] tokens: lengths and tables first-come, the lowest free pages first.  A last
+ *                       page that is not full and held by others too is copied, and the copy is the slot's.  From the first
+ *                       entry that finds too few pages on, nothing is granted and *status = CUTB_ERR_PAGES.  A slot is named once.
+ *   cutb_pages_fork     slot others[i], which must be empty, becomes a continuation of slot items[i]: it holds the same pages
+ *   cutb_pages_free     slot items[i] is empty, its pages held once less; freeing an empty slot changes nothing
+ *   cutb_pages_compact  moves the pages that are held to the places 0, 1, ..: those past the count of held pages, in their order, to
+ *                       the free places below it; tables and refs follow
+ *   cutb_pages_copy     page others[i] = page items[i]; no page may be both
+ * workspace: cutb_pages_workspace_bytes(), 256-byte aligned, of no content before or after (fork, free and copies need none).
+ */
+typedef struct cutb_pages_desc {
+  void *pages;
+  uint64_t page_bytes, ld_table;
+  uint32_t n_pages, page_tokens, n_slots, n;
+  uint32_t *tables, *lengths, *refs;
+  const uint32_t *items, *others, *counts;
+  void *workspace;
+  uint64_t workspace_bytes;
+  int *status;
+} cutb_pages_desc;
+CUTB_API uint64_t cutb_pages_workspace_bytes(const cutb_pages_desc *desc);
+CUTB_API int cutb_pages_reserve(const cutb_pages_desc *desc, void *stream);
+CUTB_API int cutb_pages_fork(const cutb_pages_desc *desc, void *stream);
+CUTB_API int cutb_pages_free(const cutb_pages_desc *desc, void *stream);
+CUTB_API int cutb_pages_compact(const cutb_pages_desc *desc, void *stream);
+CUTB_API int cutb_pages_copy(const cutb_pages_desc *desc, void *stream);
+
+/*
+ * The next token of each of `rows` rows of logits (dtype CUTB_F32, CUTB_F16 or CUTB_BF16, `vocab` <= 1048576 of them, rows ld elements
+ * apart) by a given random number u[r] in [0, 1) (no counterpart in the reference).  With w_i = exp((x_i - max) / temperature), tokens
+ * ordered by falling logit, of equal ones the lower index first:
+ *   the top_k first are kept (0: all), of those the shortest beginning that has at least top_p of their weight (1 or more: all; at
+ *   least one), of those the ones with w_i >= min_p (at least one); the token is the first kept i, by index, whose sum of weights up to
+ *   and with it is above u times the sum of all kept ones.  temperature 0: the largest logit.
+ * temperature, top_k, top_p, min_p: a value per row in device memory; null: 1, 0, 1, 0.  logprobs (optional): the logarithm of the
+ * token's share of the kept weight.  Weights are sums of 2^-42 of the largest, exactly added: the order of the additions is of no
+ * account.  A NaN counts as minus infinity; if the largest is plus infinity, its places share the weight.  A row with no
+ * logit above minus infinity gives CUTB_NO_TOKEN and minus infinity.  A temperature that is negative or not finite, a NaN among the settings or
+ * a u outside [0, 1) gives the same and sets *status to CUTB_ERR_INVALID.
+ */
+typedef struct cutb_sample_desc {
+  const void *logits;
+  uint64_t ld;
+  uint32_t rows, vocab;
+  int32_t dtype;
+  const float *temperature;
+  const uint32_t *top_k;
+  const float *top_p, *min_p, *u;
+  uint32_t *tokens;
+  float *logprobs;
+  int *status;
+} cutb_sample_desc;
+CUTB_API int cutb_sample(const cutb_sample_desc *desc, void *stream);
 
 CUTB_API int cutb_version(void);
 CUTB_API const char *cutb_status_string(int status);

@@ -1,0 +1,344 @@
+"""The paged 4-bit cache on the GPU: rows written and read back (the bytes too), attention over it, against a plain model in 64 bits."""
+import numpy as np
+import pytest
+
+import paged_util as P
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def cuda(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def make_cache(lengths, kv, head, page, r, n_layers=1, layer=0, spare=2, fill=255):
+    """A cache whose sequences hold pages in a random order; every byte of the pool is `fill` (as fp16 numbers NaN)."""
+    from cut_b200.paged import PagedCache
+
+    need = [-(-n // page) for n in lengths]
+    order = r.permutation(sum(need) + spare)
+    c = PagedCache.allocate(sum(need) + spare, len(lengths), max(1, max(need) + 1) * page, kv, head, n_layers=n_layers, page_tokens=page)
+    t, at = -np.ones(tuple(c.tables.shape), dtype=np.int32), 0
+    for s, k in enumerate(need):
+        t[s, :k] = order[at: at + k]
+        at += k
+    c.tables.copy_(cuda(t))
+    c.lengths.copy_(cuda(np.array(lengths, dtype=np.int32)))
+    c.pages.fill_(fill)
+    return c
+
+
+def rows_of(new):
+    return cuda(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+
+
+def fill_cache(c, lengths, kv, head, r, spread=1.0):
+    """Writes every token; returns the values that the cache holds, [kv, tokens, head] for each sequence."""
+    from cut_b200 import ops
+
+    n = sum(lengths)
+    if n == 0:
+        return [np.zeros((kv, 0, head)) for _ in lengths], [np.zeros((kv, 0, head)) for _ in lengths]
+    k, v = (spread * r.standard_normal((n, kv * head))).astype(np.float32), r.standard_normal((n, kv * head)).astype(np.float32)
+    ops.paged_kv_write(c, cuda(k), cuda(v), starts=rows_of(lengths))
+    cut = np.cumsum([0] + list(lengths))
+    out = [[P.quantised(x.reshape(n, kv, head)[a:b])[0].transpose(1, 0, 2) for a, b in zip(cut, cut[1:])] for x in (k, v)]
+    return out[0], out[1]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("head,kv,page,rot,pairing", [(128, 2, 64, 128, 0), (64, 1, 16, 32, 1), (40, 3, 32, 40, 0), (192, 2, 16, 64, 1), (256, 1, 128, 256, 0),
+                                                      (33, 2, 16, 0, 0), (1, 1, 256, 0, 0), (80, 1, 16, 6, 0), (128, 1, 64, 2, 1)])
+def test_written_rows_and_their_bytes(kind, head, kv, page, rot, pairing):
+    from cut_b200 import ops
+
+    r = np.random.default_rng(head + page)
+    lengths, new, heads = [1, 37, 20, page + 1, 5], [1, 30, 0, page + 1, 2], 2 * kv
+    c = make_cache(lengths, kv, head, page, r)
+    before = c.pages.cpu().numpy().copy()
+    n, t = sum(new), TYPES[kind]
+    qkv = (3 * torch.from_numpy(r.standard_normal((n + 2, (heads + 2 * kv) * head)))).to(t).cuda()  # two rows behind the last sequence
+    q, k, v = qkv[:, : heads * head], qkv[:, heads * head: (heads + kv) * head], qkv[:, (heads + kv) * head:]  # (strided)
+    cos, sin = P.tables_of(head, rot, 300)
+    q_out = torch.full((n + 2, heads * head), 7.0, dtype=t, device="cuda")
+    kw = dict(rot_dims=rot, pairing=pairing, cos_t=cuda(cos), sin_t=cuda(sin)) if rot else {}
+    ops.paged_kv_write(c, k, v, q=q, q_out=q_out, starts=rows_of(new), **kw)
+    c.check()
+    ko, vo = ops.paged_kv_read(c, n + 2, starts=rows_of(new), dtype=torch.float32)
+    c.check()
+    x = qkv.float().cpu().numpy()
+    pool, tables = c.pages.cpu().numpy(), c.tables.cpu().numpy()
+    want_k, want_v, row, touched = [], [], 0, np.zeros(pool.shape, dtype=bool)
+    unit_bytes = 20 * P.pad(head)
+    for s, m in enumerate(new):
+        for i in range(m):
+            pos = lengths[s] - m + i
+            heads_x = P.turned(x[row, : (heads + kv) * head].reshape(-1, head), pos, cos, sin, rot, pairing)
+            got_q = q_out[row].float().cpu().numpy()
+            assert np.array_equal(got_q, torch.from_numpy(heads_x[:heads].reshape(-1)).to(t).float().numpy())
+            want_k.append(P.quantised(heads_x[heads:])[0].reshape(-1))
+            want_v.append(P.quantised(x[row, (heads + kv) * head:].reshape(kv, head))[0].reshape(-1))
+            for h in range(kv):
+                at = (h * (page // 16) + pos % page // 16) * unit_bytes
+                touched[tables[s, pos // page], at: at + unit_bytes] = True
+            if i % 7 == 0:  # the bytes, as the layout says
+                at = (kv - 1) * (page // 16) * unit_bytes + pos % page // 16 * unit_bytes
+                unit = pool[tables[s, pos // page], at: at + unit_bytes]
+                assert np.array_equal(P.unit_values(unit, head, "k")[pos % 16], want_k[-1][(kv - 1) * head:])
+                assert np.array_equal(P.unit_values(unit, head, "v")[pos % 16], want_v[-1][(kv - 1) * head:])
+            row += 1
+    assert np.array_equal(ko[:n].cpu().numpy(), np.array(want_k)) and np.array_equal(vo[:n].cpu().numpy(), np.array(want_v))
+    assert not ko[n:].any() and not vo[n:].any() and bool((q_out[n:] == 7).all())
+    assert np.array_equal(pool[~touched], before[~touched])
+
+
+def test_values_that_the_cache_cannot_hold():
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(0)
+    c = make_cache([3], 1, 64, 16, r)
+    x = r.standard_normal((3, 64)).astype(np.float32)
+    x[0, 5], x[0, 40], x[1, 3], x[1, 33], x[2, :32], x[2, 32:] = np.inf, -1e30, np.nan, 7e4, 2.5, 1e-9
+    ops.paged_kv_write(c, cuda(x), cuda(x), starts=rows_of([3]))
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_RANGE
+    k, v = ops.paged_kv_read(c, 3, starts=rows_of([3]), dtype=torch.float32)
+    want, changed = P.quantised(x)
+    assert changed and np.isfinite(want).all() and np.array_equal(k.cpu().numpy(), want) and torch.equal(k, v)
+    c.check()
+
+
+CASES = [  # head, query heads, kv heads, page, lengths, new rows, window
+    (128, 8, 2, 64, [1, 15, 16, 17, 64, 65, 300], [1] * 7, 0),
+    (128, 8, 1, 16, [200, 33], [1, 1], 0),
+    (128, 4, 4, 16, [70, 0, 129], [1, 0, 1], 0),
+    (64, 6, 2, 32, [50, 100], [1, 1], 20),
+    (40, 3, 1, 16, [31, 90], [1, 1], 0),
+    (192, 14, 2, 16, [40, 21], [1, 1], 7),
+    (256, 16, 1, 64, [100, 3], [1, 1], 0),
+    (96, 24, 1, 32, [77], [1], 0),
+    (128, 8, 2, 64, [40, 130, 9], [3, 5, 2], 0),
+    (128, 32, 8, 64, [200, 70, 33], [150, 70, 1], 0),
+    (128, 4, 2, 16, [333], [333], 0),
+    (64, 4, 4, 16, [290, 60], [129, 60], 33),
+    (256, 4, 1, 32, [150], [100], 0),
+    (80, 5, 5, 16, [140, 12], [139, 12], 1),
+    (192, 2, 2, 128, [260], [130], 100),
+    (128, 20, 1, 64, [90], [50], 0),
+]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("head,nh,kv,page,lengths,new,window", CASES)
+def test_attention(kind, head, nh, kv, page, lengths, new, window):
+    from cut_b200 import ops
+
+    r = np.random.default_rng(head + nh + len(lengths))
+    c = make_cache(lengths, kv, head, page, r)
+    ks, vs = fill_cache(c, lengths, kv, head, r, spread=2.0)
+    n, t = sum(new), TYPES[kind]
+    q = torch.from_numpy(1.5 * r.standard_normal((n + 3, nh * head))).to(t).cuda()  # three rows behind the last sequence
+    out = torch.full((n + 3, nh * head), 7.0, dtype=t, device="cuda")
+    ops.paged_attention(c, q, nh, starts=rows_of(new), max_new=max(new), window=window, out=out)
+    c.check()
+    x, got, row, scale = q.double().cpu().numpy(), out.double().cpu().numpy(), 0, float(np.float32(head ** -0.5))
+    for s, m in enumerate(new):
+        for i in range(m):
+            for h in range(nh):
+                y, spread, products = P.attention(x[row, h * head: (h + 1) * head], ks[s][h * kv // nh], vs[s][h * kv // nh], lengths[s] - m + i, scale, window)
+                off = np.abs(got[row, h * head: (h + 1) * head] - y) - P.tolerance(y, spread, products, scale, kind)
+                assert off.max() <= 0, (s, i, h, off.max(), int(off.argmax()))
+            row += 1
+    assert bool((out[n:] == 7).all())
+
+
+def test_one_row_each_slots_layers_and_strides():
+    """Sequences by slot in an order of their own, one row each; the second layer of a cache; rows inside a wider matrix."""
+    from cut_b200 import ops
+
+    r = np.random.default_rng(5)
+    lengths, kv, head, nh = [20, 60, 33, 90], 2, 64, 4
+    c = make_cache(lengths, kv, head, 16, r, n_layers=3)
+    part = c.layer_bytes()
+    from cut_b200.paged import PagedCache
+
+    second = PagedCache(c.pages[:, part: 2 * part], c.tables, c.lengths, c.refs, page_tokens=16, n_kv_heads=kv, head_dim=head, status=c.status)
+    ks, vs = fill_cache(second, lengths, kv, head, r)
+    assert bool((c.pages[:, :part] == 255).all()) and bool((c.pages[:, 2 * part:] == 255).all())
+    wide = torch.from_numpy(r.standard_normal((2, nh * head + 24)).astype(np.float32)).cuda()
+    q, slots = wide[:, 8: 8 + nh * head], [3, 1]
+    out = ops.paged_attention(c, q, nh, slots=cuda(np.array(slots, dtype=np.int32)), layer=1, scale=-0.3)
+    c.check()
+    x, got = q.double().cpu().numpy(), out.double().cpu().numpy()
+    for i, s in enumerate(slots):
+        for h in range(nh):
+            y, spread, products = P.attention(x[i, h * head: (h + 1) * head], ks[s][h // 2], vs[s][h // 2], lengths[s] - 1, float(np.float32(-0.3)), 0)
+            assert (np.abs(got[i, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, 0.3, "f32")).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_bad_pages_slots_and_lengths_are_left_out_and_reported(new):
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(6)
+    lengths, kv, head, nh = [60, 60, 60, 60, 60, 60], 1, 64, 2
+    c = make_cache(lengths, kv, head, 16, r)
+    ks, vs = fill_cache(c, lengths, kv, head, r)
+    c.check()
+    c.tables[1, 1] = 1 << 20           # a page that does not exist: its keys are not there
+    c.lengths[2] = 1 << 30             # longer than the table
+    c.lengths[3] = new - 1             # shorter than the new rows
+    slots = cuda(np.array([0, 1, 2, 3, 77, 5], dtype=np.int32))
+    q = torch.from_numpy(r.standard_normal((6 * new, nh * head)).astype(np.float32)).cuda()
+    starts = rows_of([new] * 6)
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention(c, q, nh, starts=starts, slots=slots, max_new=new, out=out)
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_INVALID
+    x, got = q.double().cpu().numpy(), out.double().cpu().numpy()
+    assert (got[2 * new: 5 * new] == 7).all()
+    for s in (0, 1, 5):
+        keep = np.r_[0:16, 32:60] if s == 1 else np.r_[0:60]
+        for i in (0, new - 1):
+            pos = 60 - new + i
+            seen = keep[keep <= pos]
+            for h in range(nh):
+                y, spread, products = P.attention(x[s * new + i, h * head: (h + 1) * head], ks[s][0][seen], vs[s][0][seen], len(seen) - 1, 0.125, 0)
+                assert (np.abs(got[s * new + i, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, 0.125, "f32")).all(), (s, i, h)
+    # the same to be written: nothing of it is touched, the others are
+    before = c.pages.clone()
+    k = torch.from_numpy(r.standard_normal((6 * new, head)).astype(np.float32)).cuda()
+    c.tables[0, 3] = -5  # (the last page of slot 0)
+    ops.paged_kv_write(c, k, k, starts=starts, slots=slots, max_new=new)
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_INVALID
+    changed = (c.pages != before).any(1).nonzero().view(-1).tolist()
+    own = set(c.tables[5, :4].tolist()) | set(c.tables[1, 2:4].tolist()) | (set(c.tables[0, 1:3].tolist()) | {int(c.tables[1, 0])} if new > 1 else set())
+    assert set(changed) <= own and int(c.tables[5, 3]) in changed
+
+
+def test_positions_past_the_tables_and_rows_past_the_call():
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(7)
+    c = make_cache([20, 20], 1, 64, 16, r)
+    cos, sin = P.tables_of(64, 64, 18)
+    k = torch.from_numpy(r.standard_normal((6, 64)).astype(np.float32)).cuda()
+    ops.paged_kv_write(c, k, k, starts=rows_of([3, 3]), rot_dims=64, cos_t=cuda(cos), sin_t=cuda(sin))  # positions 17, 18, 19
+    with pytest.raises(L.CutbError):
+        c.check()
+    ko, _ = ops.paged_kv_read(c, 6, starts=rows_of([3, 3]), dtype=torch.float32)
+    assert np.isfinite(ko.cpu().numpy()[[0, 3]]).all() and np.isnan(ko.cpu().numpy()[[1, 2, 4, 5]]).all()
+    for starts, max_new in (([0, 4, 9], 8), ([0, 2, 1], 8), ([0, 3, 6], 2)):  # behind the rows, falling, more than max_new
+        out = torch.full((6, 64), 7.0, device="cuda")
+        c.pages.zero_()
+        ops.paged_attention(c, torch.ones(6, 64, device="cuda"), 1, starts=cuda(np.array(starts, dtype=np.int32)), max_new=max_new, out=out)
+        with pytest.raises(L.CutbError):
+            c.check()
+        assert bool((out[4:] == 7).all())
+
+
+def test_scores_that_jump_and_a_zero_scale():
+    """Large scores that rise along the keys (the running maximum follows), and a scale of zero (the mean of the values)."""
+    from cut_b200 import ops
+
+    r = np.random.default_rng(8)
+    n, head = 700, 128
+    c = make_cache([n], 1, head, 64, r)
+    direction = r.standard_normal(head)
+    k = (np.linspace(-6, 6, n)[:, None] * direction + 0.1 * r.standard_normal((n, head))).astype(np.float32)
+    v = r.standard_normal((n, head)).astype(np.float32)
+    ops.paged_kv_write(c, cuda(k), cuda(v), starts=rows_of([n]))
+    kq, vq = P.quantised(k)[0], P.quantised(v)[0]
+    for rows in (1, 200):
+        q = np.tile(direction.astype(np.float32), (rows, 4))
+        q[:, head:] *= np.float32(-1)
+        for scale in (1.0, 0.0):
+            out = ops.paged_attention(c, cuda(q), 4, starts=rows_of([rows]), max_new=rows, scale=scale).double().cpu().numpy()
+            for i in {0, rows - 1}:
+                for h in (0, 1):
+                    y, spread, products = P.attention(q[i, h * head: (h + 1) * head].astype(np.float64), kq, vq, n - rows + i, scale, 0)
+                    assert (np.abs(out[i, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, scale, "f32")).all(), (rows, scale, i, h)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_long_sequences_share_their_work(kind):
+    from cut_b200 import ops
+
+    r = np.random.default_rng(9)
+    lengths, kv, head, nh = [20000, 17, 5000], 1, 128, 4
+    c = make_cache(lengths, kv, head, 64, r)
+    ks, vs = fill_cache(c, lengths, kv, head, r)
+    q = torch.from_numpy(r.standard_normal((3, nh * head))).to(TYPES[kind]).cuda()
+    got = ops.paged_attention(c, q, nh).double().cpu().numpy()
+    again = ops.paged_attention(c, q, nh).double().cpu().numpy()
+    assert np.array_equal(got, again)
+    x, scale = q.double().cpu().numpy(), float(np.float32(head ** -0.5))
+    for s in range(3):
+        for h in range(nh):
+            y, spread, products = P.attention(x[s, h * head: (h + 1) * head], ks[s][0], vs[s][0], lengths[s] - 1, scale, 0)
+            assert (np.abs(got[s, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, scale, kind)).all(), (s, h)
+
+
+def test_offsets_past_32_bits():
+    """A pool of over 4 GB, the sequence in its last pages."""
+    from cut_b200 import ops
+    from cut_b200.paged import PagedCache
+
+    r = np.random.default_rng(10)
+    c = PagedCache.allocate(4200, 1, 256, 1, 128, page_tokens=64)
+    pages = torch.zeros((4200, 1 << 20), dtype=torch.uint8, device="cuda")
+    c = PagedCache(pages, c.tables, c.lengths, c.refs, page_tokens=64, n_kv_heads=1, head_dim=128, status=c.status)
+    c.tables[0, :3] = torch.tensor([4199, 1, 4198], dtype=torch.int32)
+    c.lengths[0] = 150
+    ks, vs = fill_cache(c, [150], 1, 128, r)
+    q = torch.from_numpy(r.standard_normal((1, 256)).astype(np.float32)).cuda()
+    got = ops.paged_attention(c, q, 2).double().cpu().numpy()
+    for h in range(2):
+        y, spread, products = P.attention(q.double().cpu().numpy()[0, h * 128: (h + 1) * 128], ks[0][0], vs[0][0], 149, 128 ** -0.5, 0)
+        assert (np.abs(got[0, h * 128: (h + 1) * 128] - y) <= P.tolerance(y, spread, products, 128 ** -0.5, "f32")).all()
+    c.check()
+
+
+def test_recorded_calls_follow_the_lengths_and_streams_stay_apart():
+    """A step recorded once serves later steps; two recorded calls with workspaces of their own run on two streams."""
+    from cut_b200 import ops
+
+    r = np.random.default_rng(11)
+    kv, head, nh = 2, 128, 8
+    lengths = [400, 100]
+    c = make_cache([500, 500], kv, head, 64, r)
+    ks, vs = fill_cache(c, [500, 500], kv, head, r)
+    q = torch.from_numpy(r.standard_normal((2, nh * head)).astype(np.float32)).cuda()
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for out, st in zip(outs, streams):
+        with torch.cuda.stream(st):
+            ops.paged_attention(c, q, nh, out=out)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                ops.paged_attention(c, q, nh, out=out)
+            graphs.append(g)
+    for lengths in ([400, 100], [7, 500], [500, 1]):
+        c.lengths.copy_(cuda(np.array(lengths, dtype=np.int32)))
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+        got, x = outs[0].double().cpu().numpy(), q.double().cpu().numpy()
+        for s in range(2):
+            for h in (0, nh - 1):
+                y, spread, products = P.attention(x[s, h * head: (h + 1) * head], ks[s][h * kv // nh], vs[s][h * kv // nh], lengths[s] - 1, 128 ** -0.5, 0)
+                assert (np.abs(got[s, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, 128 ** -0.5, "f32")).all()

@@ -1,0 +1,133 @@
+"""Sampling on the GPU against the same in 64 bits: every choice equal, the logarithms to fp32's last digits."""
+import numpy as np
+import pytest
+
+import paged_util as P
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def run(x, u, t=None, k=None, p=None, least=None):
+    """x: torch logits on the GPU; the settings as lists or None -> (tokens, logprobs, status)"""
+    from cut_b200 import ops
+
+    dev = lambda v, kind: None if v is None else torch.tensor(np.asarray(v), dtype=kind).cuda()  # noqa: E731
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tokens, logs = ops.sample(x, dev(u, torch.float32), temperature=dev(t, torch.float32), top_k=dev(k, torch.int32), top_p=dev(p, torch.float32),
+                              min_p=dev(least, torch.float32), want_logprobs=True, status=st)
+    return tokens.cpu().numpy(), logs.cpu().numpy(), int(st.item())
+
+
+def check(x, u, t=None, k=None, p=None, least=None):
+    n = len(u)
+    got, logs, st = run(x, u, t, k, p, least)
+    assert st == 0
+    rows = x.double().cpu().numpy()
+    f = lambda v, d: np.full(n, d) if v is None else np.asarray(v, dtype=np.float32).astype(np.float64)  # noqa: E731
+    for r in range(n):
+        tok, lp = P.sampled(rows[r], f(t, 1)[r], 0 if k is None else k[r], f(p, 1)[r], f(least, 0)[r], float(np.float32(u[r])))
+        assert got[r] == (-1 if tok is None else tok), r
+        # the shares are within 2^-40, the logarithm is rounded once
+        assert (lp == logs[r]) or abs(logs[r] - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -36, (r, logs[r], lp)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab", [1, 2, 31, 1000, 32000, 50257, 128256])
+def test_settings(kind, vocab):
+    r = np.random.default_rng(vocab)
+    n = 24
+    x = torch.from_numpy(2.5 * r.standard_normal((n, vocab))).to(TYPES[kind]).cuda()
+    x[::2, : max(1, vocab // 7)] += 5
+    u = r.random(n).astype(np.float32)
+    t, k = r.choice([0, 0.01, 0.7, 1, 1.3, 5], n), r.choice([0, 1, 5, 50, vocab - 1, vocab, vocab + 9], n).astype(int)
+    p, least = r.choice([1.0, 0.0, 0.5, 0.9, 0.999, 2.0, -1.0], n), r.choice([0, 0, 1e-4, 0.05, 0.3, 1.0, 7.0], n)
+    check(x, u)
+    check(x, u, t=t)
+    check(x, u, k=k)
+    check(x, u, p=p)
+    check(x, u, least=least)
+    check(x, u, t, k, p, least)
+
+
+def test_ties_and_ends_of_the_range():
+    """Equal logits are taken in their order; u of zero and just below one; zeros of both signs are equal."""
+    x = torch.zeros(12, 1000, device="cuda")
+    x[1::2, ::3] = -0.0
+    u = np.array([0, 1 - 2 ** -24, 0.5, 0.25, 0.125, 0.999, 0.3, 0.7, 0, 0.9999, 1e-30, 0.0625], dtype=np.float32)
+    check(x, u)
+    check(x, u, k=[1, 2, 3, 10, 33, 999, 1000, 500, 1, 7, 64, 5])
+    check(x, u, p=[0.1, 0.5, 1e-9, 0.0105, 0.25, 0.75, 0.999, 0.0, 0.3, 0.2, 0.9, 0.0625])
+    check(x, u, k=[100] * 12, p=[0.25] * 12)
+    check(x, u, t=[0.0] * 12)
+    x[:, 400:] = 3.0
+    check(x, u, k=[600, 601, 599, 10, 700, 650, 1, 0, 900, 620, 3, 605], p=[1, 0.99, 0.5] * 4)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_masked_and_not_finite(kind):
+    r = np.random.default_rng(1)
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(TYPES[kind]).min
+    x = torch.from_numpy(r.standard_normal((8, 500))).to(TYPES[kind]).cuda()
+    x[0, 3:] = -inf
+    x[1, ::2] = nan
+    x[2, [7, 70, 400]] = inf
+    x[3] = -inf
+    x[4] = nan
+    x[5, :490] = low
+    x[6] = low
+    x[7, 5], x[7, 6] = inf, nan
+    u = r.random(8)
+    check(x, u)
+    check(x, u, t=[0.5] * 8, k=[20] * 8, p=[0.9] * 8, least=[0.01] * 8)
+    check(x, u, t=[0.0] * 8)
+    check(x, u, k=[500, 499, 2, 1, 1, 495, 3, 2])
+
+
+def test_settings_that_mean_nothing():
+    from cut_b200 import _lib as L
+
+    x = torch.randn(9, 50, device="cuda")
+    nan, inf = float("nan"), float("inf")
+    u, t, p, least = [0.5] * 9, [1.0] * 9, [0.9] * 9, [0.1] * 9
+    u[0], u[1], u[2], t[3], t[4], t[5], p[6], least[7] = 1.0, -0.1, nan, -1.0, nan, inf, nan, nan
+    got, logs, st = run(x, u, t, None, p, least)
+    assert st == L.ERR_INVALID and (got[:8] == -1).all() and (logs[:8] == -np.inf).all() and 0 <= got[8] < 50
+
+
+def test_many_choices_of_one_row():
+    """The tokens that u from 0 to 1 gives, one after another, have the weights' shares."""
+    r = np.random.default_rng(4)
+    row = torch.from_numpy((3 * r.standard_normal(5000)).astype(np.float32)).cuda()
+    n = 2000
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    x = row.expand(n, -1).contiguous()
+    check(x, u)
+    check(x, u, k=[100] * n, p=[0.8] * n)
+
+
+def test_strides_offsets_streams_and_recordings():
+    from cut_b200 import ops
+
+    r = np.random.default_rng(5)
+    wide = torch.from_numpy(r.standard_normal((5, 4099)).astype(np.float32)).cuda()
+    for off in (0, 1, 2, 3):
+        check(wide[:, off: off + 4001], r.random(5))
+    half = wide.bfloat16()
+    for off in (1, 2, 7):
+        check(half[:, off: off + 4003], r.random(5), k=[50] * 5)
+    u = torch.rand(5, device="cuda")
+    tokens, s = torch.zeros(5, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.sample(wide, u, tokens=tokens)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ops.sample(wide, u, tokens=tokens)
+    for _ in range(3):
+        u.copy_(torch.rand(5))
+        g.replay()
+        torch.cuda.synchronize()
+        assert tokens.tolist() == [P.sampled(row, 1.0, 0, 1.0, 0.0, a)[0] for row, a in zip(wide.double().cpu().numpy(), u.double().cpu().numpy())]

@@ -1,0 +1,153 @@
+"""Refusals of the paged cache's and the sampler's entry points: host logic, answered without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from cut_b200 import _lib as L
+from cut_b200 import ops
+from cut_b200.paged import PagedCache
+
+
+def desc(**kw):
+    d = L.PagedDesc()
+    base = dict(pages=4096, page_bytes=81920, ld_table=8, n_pages=4, page_tokens=64, n_kv_heads=8, head_dim=128, tables=256, lengths=256,
+                n_slots=2, n_seqs=2, n_tokens=2, max_new=1, dtype=L.F32, n_heads=32, q=256, ldq=4096, k=256, ldk=1024, v=256, ldv=1024,
+                q_out=512, ldq_out=4096, k_out=256, ldk_out=1024, v_out=256, ldv_out=1024, out=256, ldo=4096, scale=0.1)
+    for k, v in {**base, **kw}.items():
+        setattr(d, k, v)
+    return d
+
+
+def refused(name, d, word, code=L.ERR_INVALID):
+    lib = L.lib()
+    assert getattr(lib, name)(C.byref(d) if d is not None else None, None) == code, (name, word, lib.cutb_last_error())
+    assert word in lib.cutb_last_error().decode(), (word, lib.cutb_last_error())
+
+
+CALLS = ("cutb_paged_kv_write", "cutb_paged_kv_read", "cutb_paged_attention")
+
+
+def test_struct_sizes_are_the_headers():
+    assert (C.sizeof(L.PagedDesc), C.sizeof(L.PagesDesc), C.sizeof(L.SampleDesc)) == (272, 112, 96)
+
+
+def test_layer_bytes():
+    f = L.lib().cutb_paged_layer_bytes
+    assert f(8, 128, 64) == 8 * 4 * 20 * 128 and f(1, 1, 16) == 20 * 64 and f(3, 129, 256) == 3 * 16 * 20 * 192
+    assert f(8, 128, 48) == f(8, 128, 8) == f(8, 128, 512) == f(0, 128, 64) == f(8, 257, 64) == f(8, 0, 64) == 0
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("kw,word", [({"dtype": 7}, "element type"), ({"page_tokens": 48}, "a page holds"), ({"head_dim": 257}, "a page holds"),
+                                     ({"head_dim": 0}, "a page holds"), ({"n_pages": 0}, "a page holds"), ({"ld_table": 0}, "a page holds"),
+                                     ({"pages": None}, "null pointer"), ({"pages": 4104}, "16-byte"), ({"page_bytes": 81904}, "short of"),
+                                     ({"page_bytes": 81928}, "16-byte"), ({"tables": None}, "null pointer"), ({"lengths": None}, "null pointer"),
+                                     ({"n_seqs": 3, "n_tokens": 3}, "sequences"), ({"n_tokens": 1}, "sequences"), ({"max_new": 0}, "max_new"),
+                                     ({"n_seqs": 4097, "slots": 256, "n_tokens": 4097}, "sequences"), ({"ld_table": 1 << 30}, "31 bits")])
+def test_caches_and_sequences_that_are_refused(name, kw, word):
+    refused(name, desc(**kw), word)
+
+
+def test_rows_that_are_refused():
+    for name in CALLS:
+        refused(name, None, "null descriptor")
+        assert getattr(L.lib(), name)(C.byref(desc(n_tokens=0, n_seqs=0)), None) == L.OK  # nothing to do
+    refused("cutb_paged_kv_write", desc(k=None), "rows")
+    refused("cutb_paged_kv_write", desc(v=258), "rows")
+    refused("cutb_paged_kv_write", desc(ldk=1023), "rows")
+    refused("cutb_paged_kv_write", desc(n_heads=12), "multiple")
+    refused("cutb_paged_kv_write", desc(q_out=None), "rows")
+    refused("cutb_paged_kv_write", desc(rot_dims=3), "rot_dims")
+    refused("cutb_paged_kv_write", desc(rot_dims=130, cos_table=256, sin_table=256, max_pos=9), "rot_dims")
+    refused("cutb_paged_kv_write", desc(rot_dims=128), "tables")
+    refused("cutb_paged_kv_write", desc(rot_dims=128, cos_table=256, sin_table=256, max_pos=9, rot_pairing=2), "pairing")
+    refused("cutb_paged_kv_write", desc(rot_dims=128, cos_table=256, sin_table=256, max_pos=9, q_out=256), "of their own")
+    refused("cutb_paged_kv_read", desc(v_out=None), "rows")
+    refused("cutb_paged_attention", desc(n_heads=0), "multiple")
+    refused("cutb_paged_attention", desc(out=None), "rows")
+    refused("cutb_paged_attention", desc(ldq=4095), "rows")
+    refused("cutb_paged_attention", desc(scale=float("nan")), "finite")
+    refused("cutb_paged_attention", desc(scale=float("inf")), "finite")
+    assert L.lib().cutb_paged_workspace_bytes(C.byref(desc(page_tokens=48))) == 0
+
+
+def pages(**kw):
+    d = L.PagesDesc()
+    base = dict(pages=4096, page_bytes=4096, ld_table=8, n_pages=4, page_tokens=64, n_slots=2, n=1, tables=256, lengths=256, refs=256, items=256,
+                others=256, counts=256, workspace=4096, workspace_bytes=1 << 20)
+    for k, v in {**base, **kw}.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_bookkeeping_that_is_refused():
+    for name in ("reserve", "fork", "free", "compact"):
+        for kw in ({"tables": None}, {"lengths": None}, {"refs": None}, {"n_pages": 0}, {"n_slots": 0}, {"page_tokens": 12}, {"ld_table": 1 << 30}):
+            refused("cutb_pages_" + name, pages(**kw), "a page that does not hold")
+    for name in ("reserve", "compact", "copy"):
+        for kw in ({"pages": None}, {"pages": 4104}, {"page_bytes": 4104}, {"page_bytes": 0}):
+            refused("cutb_pages_" + name, pages(**kw), "16-byte")
+    for name in ("reserve", "fork", "free"):
+        refused("cutb_pages_" + name, pages(n=1025), "1024")
+        refused("cutb_pages_" + name, pages(items=None), "null entries")
+        assert getattr(L.lib(), "cutb_pages_" + name)(C.byref(pages(n=0)), None) == L.OK
+    refused("cutb_pages_copy", pages(n=65536), "65535")
+    refused("cutb_pages_copy", pages(others=None), "null entries")
+    refused("cutb_pages_reserve", pages(counts=None), "null entries")
+    for name in ("reserve", "compact"):
+        refused("cutb_pages_" + name, pages(workspace_bytes=64), "workspace", L.ERR_WORKSPACE)
+        refused("cutb_pages_" + name, pages(workspace=4100), "workspace", L.ERR_WORKSPACE)
+    assert L.lib().cutb_pages_workspace_bytes(C.byref(pages())) >= 256 and L.lib().cutb_pages_workspace_bytes(None) == 0
+    assert L.lib().cutb_status_string(L.ERR_PAGES) == b"too few free pages"
+
+
+def test_sampling_that_is_refused():
+    def s(**kw):
+        d = L.SampleDesc()
+        for k, v in {**dict(logits=256, ld=100, rows=2, vocab=100, dtype=L.F32, u=256, tokens=256), **kw}.items():
+            setattr(d, k, v)
+        return d
+
+    refused("cutb_sample", None, "null descriptor")
+    refused("cutb_sample", s(dtype=3), "element type")
+    refused("cutb_sample", s(vocab=0), "logits")
+    refused("cutb_sample", s(vocab=(1 << 20) + 1, ld=1 << 21), "logits")
+    refused("cutb_sample", s(ld=99), "stride")
+    refused("cutb_sample", s(u=None), "null")
+    refused("cutb_sample", s(tokens=None), "null")
+    refused("cutb_sample", s(logits=258), "misaligned")
+    assert L.lib().cutb_sample(C.byref(s(rows=0)), None) == L.OK
+
+
+def test_python_refuses_tensors_that_are_not_on_the_device_or_not_alike():
+    z = lambda *shape, t=torch.int32: torch.zeros(shape, dtype=t)  # noqa: E731
+    with pytest.raises(RuntimeError, match="uint8"):
+        PagedCache(z(4, 64), z(2, 2), z(2), z(4))
+    with pytest.raises(RuntimeError, match="per table row"):
+        PagedCache(z(4, 64, t=torch.uint8), z(2, 2), z(3), z(4))
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        PagedCache(z(4, 72, t=torch.uint8), z(2, 2), z(2), z(4))
+    with pytest.raises(ValueError):
+        PagedCache.allocate(4, 2, 64, 8, 257, device="cpu")
+    c = PagedCache.allocate(4, 2, 200, 2, 32, n_layers=3, page_tokens=16, device="cpu")
+    assert c.pages.shape == (4, 3 * 2 * 20 * 64) and c.tables.shape == (2, 13) and int(c.tables.max()) == -1 and c.layer_bytes() == 2 * 20 * 64
+    f = lambda n: torch.zeros(1, n)  # noqa: E731
+    with pytest.raises(RuntimeError, match="rows of 2 x 32"):
+        ops.paged_kv_write(c, f(63), f(64))
+    with pytest.raises(RuntimeError, match="one type"):
+        ops.paged_kv_write(c, f(64), f(64).half())
+    with pytest.raises(RuntimeError, match="tables"):
+        ops.paged_kv_write(c, f(64), f(64), rot_dims=32, cos_t=torch.zeros(4, 8), sin_t=torch.zeros(4, 8))
+    with pytest.raises(RuntimeError, match="current CUDA device"):
+        ops.paged_kv_write(c, f(64), f(64))
+    with pytest.raises(RuntimeError, match="current CUDA device"):
+        ops.paged_attention(c, f(128), 4)
+    with pytest.raises(RuntimeError, match="current CUDA device"):
+        c.fork([0], [1])
+    with pytest.raises(RuntimeError, match="one length"):
+        c.reserve([0, 1], [1])
+    with pytest.raises(RuntimeError, match="current CUDA device"):
+        ops.sample(torch.zeros(2, 8), torch.zeros(2))
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        ops.sample(torch.zeros(2, 8, dtype=torch.float64), torch.zeros(2))
