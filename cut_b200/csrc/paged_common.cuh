@@ -9,7 +9,7 @@ namespace cutb {
 namespace {
 
 constexpr uint32_t PG_UNIT = 16;       // tokens of a unit
-constexpr uint32_t PG_MAX_SEQS = 4096;  // sequences of a call
+constexpr uint32_t PG_MAX_SEQS = 1024;  // sequences of a call
 constexpr float PG_LIMIT = 32768.f;    // what a cached element may hold: 15 d + m stays below fp16's largest number
 
 __host__ __device__ constexpr uint32_t pg_pad(uint32_t head_dim) { return (head_dim + 63) / 64 * 64; }

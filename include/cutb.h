@@ -724,7 +724,7 @@ CUTB_API int cutb_expert_down(const cutb_expert_desc *desc, void *stream);
  * starts[i] .. starts[i + 1] - 1 (starts null: row i, one row each), at most max_new of them, n_tokens in all.  They are the last
  * rows of the sequence: row r has position lengths[slot] - (starts[i + 1] - r).  Rows behind starts[n_seqs] are neither read nor
  * written.  Element types (dtype) are CUTB_F32, CUTB_F16 or CUTB_BF16.  tables, lengths, slots and starts are device memory, read by the
- * kernels, so a recorded call serves later steps; n_seqs <= 4096.  A slot past n_slots, rows that do not fit in n_tokens, a length that
+ * kernels, so a recorded call serves later steps; n_seqs <= 1024.  A slot past n_slots, rows that do not fit in n_tokens, a length that
  * is shorter than the new rows or longer than the table, a page that does not exist and a position past max_pos set *status
  * to CUTB_ERR_INVALID; what they concern is left out (rows and keys as if they were not there), and nothing outside is touched.
  *

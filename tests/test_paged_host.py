@@ -44,7 +44,7 @@ def test_layer_bytes():
                                      ({"pages": None}, "null pointer"), ({"pages": 4104}, "16-byte"), ({"page_bytes": 81904}, "short of"),
                                      ({"page_bytes": 81928}, "16-byte"), ({"tables": None}, "null pointer"), ({"lengths": None}, "null pointer"),
                                      ({"n_seqs": 3, "n_tokens": 3}, "sequences"), ({"n_tokens": 1}, "sequences"), ({"max_new": 0}, "max_new"),
-                                     ({"n_seqs": 4097, "slots": 256, "n_tokens": 4097}, "sequences"), ({"ld_table": 1 << 30}, "31 bits")])
+                                     ({"n_seqs": 1025, "slots": 256, "n_tokens": 1025}, "sequences"), ({"ld_table": 1 << 30}, "31 bits")])
 def test_caches_and_sequences_that_are_refused(name, kw, word):
     refused(name, desc(**kw), word)
 
