@@ -5,11 +5,13 @@
 // in registers, are its A fragments, and nothing goes through shared memory twice.  P^T comes from the scores' accumulators by movmatrix.
 // 16-bit rows take 8 columns.  fp32 rows enter as two fp16 terms: a tile of 8 columns has the high parts of four rows and then their low
 // parts, and so have the weights (22 bits of each; the products are exact, the sums fp32).  Queries are scaled by a power of two so
-// that the largest element is in [1, 2), weights by 2^15: fp16 holds 2^-24 of the former and 2^-39 of the largest weight.
+// that the largest element is in [1, 2), weights are kept between 2^8
+// and 2^15 at their largest: fp16 holds 2^-24 of the former and 2^-32 of the largest weight.
 //
 // Bound by HBM: 2560 bytes of a 128-element unit are 4096 elements, and about 290 warp instructions.  Units are copied whole by bulk
 // copies, each warp through a ring of its own, so that a block has up to 80 KB in flight and warps meet only at the ends.
-// The units of all sequences and KV heads in a row are shared out evenly over the blocks.  Where a block's part begins or ends inside
+// Two units a step: what a step costs besides its products (the copy, the maximum over the lanes) is paid half as often.
+// The steps of all sequences and KV heads in a row are shared out evenly over the blocks.  Where a block's part begins or ends inside
 // a KV head's units, its maxima, sums and values go to the workspace, and a second kernel joins them in their order.
 #include "kernels.h"
 #include "paged_common.cuh"
@@ -17,30 +19,44 @@
 namespace cutb {
 namespace {
 
-constexpr uint32_t PT_WARPS = 8, PT_THREADS = 32 * PT_WARPS;
+constexpr uint32_t PT_WARPS = 8, PT_THREADS = 32 * PT_WARPS, PT_KEYS = 2 * PG_UNIT;
 
-__host__ __device__ constexpr uint32_t pt_stages(uint32_t dp) { return dp == 64 ? 8 : dp == 128 ? 4 : dp == 192 ? 3 : 2; }
-__host__ __device__ constexpr uint32_t pt_ring_bytes(uint32_t dp) { return PT_WARPS * pt_stages(dp) * pg_unit_bytes(dp); }
+__host__ __device__ constexpr uint32_t pt_stages(uint32_t dp) { return dp == 64 ? 4 : dp == 128 ? 2 : 2; }
+__host__ __device__ constexpr uint32_t pt_ring_bytes(uint32_t dp) { return PT_WARPS * pt_stages(dp) * 2 * pg_unit_bytes(dp); }
 
 struct PtSeq {
   uint32_t slot, len, row0, rows;
 };
-// The shares: block b works on the units total b / shares .. total (b + 1) / shares of all, at least PT_WARPS each.
-__device__ __forceinline__ uint32_t pt_shares(uint64_t total, uint32_t blocks) {
-  const uint64_t most = (total + PT_WARPS - 1) / PT_WARPS;
-  return (uint32_t)(most < blocks ? most : blocks);
+__device__ __forceinline__ uint64_t pt_div(uint64_t a, uint64_t b) {  // (a 64-bit division takes some hundred cycles)
+  return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
 }
-__device__ __forceinline__ uint64_t pt_from(uint64_t total, uint32_t shares, uint32_t b) { return total * b / shares; }
-// first unit that a sequence's rows see, and how many there are up to the last one
+// The shares of the blocks: `each` steps, the first `more` of them one more; at least PT_WARPS steps in each.
+struct PtShares {
+  uint64_t each, more;
+  uint32_t n;
+  __device__ __forceinline__ PtShares(uint64_t total, uint32_t blocks) {
+    const uint64_t most = (total + PT_WARPS - 1) / PT_WARPS;
+    n = (uint32_t)(most < blocks ? most : blocks);
+    each = n ? pt_div(total, n) : 0, more = total - each * n;
+  }
+  __device__ __forceinline__ uint64_t from(uint32_t b) const { return each * b + (b < more ? b : more); }
+  __device__ __forceinline__ uint32_t block_of(uint64_t x) const {
+    const uint64_t big = more * (each + 1);
+    return (uint32_t)(x < big ? pt_div(x, each + 1) : more + pt_div(x - big, each));
+  }
+};
+// first step (two units) that a sequence's rows see, and how many there are up to the last one
 __device__ __forceinline__ void pt_units(const cutb_paged_desc &d, uint32_t len, uint32_t rows, uint32_t &first, uint32_t &n) {
   const uint32_t oldest = len - rows;  // position of the first row
-  first = d.window && oldest + 1 > d.window ? (oldest + 1 - d.window) / PG_UNIT : 0;
-  n = (len + PG_UNIT - 1) / PG_UNIT - first;
+  first = d.window && oldest + 1 > d.window ? (oldest + 1 - d.window) / PT_KEYS : 0;
+  n = (len + PT_KEYS - 1) / PT_KEYS - first;
 }
 
 struct PtPlan {
   uint32_t rows;       // query rows of an item
   uint32_t blocks;     // at most
+  uint32_t vec;        // the queries may be read 16 bytes at a time
+  float scale, sign;   // |scale| log2(e), and its sign, which goes to the queries (a scale of zero: queries of zero)
   uint64_t *prefix;    // workspace: units (times rows' chunks) of the sequences before
   float *part;         // workspace: [block][2][rows][dp + 2]
 };
@@ -70,12 +86,13 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
   uint64_t *prefix = reinterpret_cast<uint64_t *>(pt_smem + pt_ring_bytes(DP));
   PtSeq *seqs = reinterpret_cast<PtSeq *>(prefix + d.n_seqs + 1);
   __shared__ __align__(8) uint64_t bars[PT_WARPS * S];
-  __shared__ float m_s[PT_WARPS][8 * NT], l_s[PT_WARPS][8 * NT];
+  __shared__ __align__(16) float2 part_s[8 * NT][PT_WARPS];  // of a column and a warp: what its weights are relative to, their sum
   __shared__ uint64_t sums[PT_WARPS], carry_s;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane / 4, t = lane % 4;
-  const uint32_t bar = smem_u32(bars) + warp * S * 8, ring = smem_u32(pt_smem) + warp * S * UB;
+  const uint32_t bar = smem_u32(bars) + warp * S * 8, ring = smem_u32(pt_smem) + warp * S * 2 * UB;
+  const uint32_t page_units = d.page_tokens / PG_UNIT, page_mask = page_units - 1, page_shift = 31 - __clz(page_units);
   if (lane == 0) {
-    for (uint32_t i = 0; i < S; ++i) mbar_init(bar + 8 * i, 1);
+    for (uint32_t i = 0; i < S; ++i) mbar_init(bar + 8 * i, 2);
     fence_mbar_init();
   }
   pdl_enter();
@@ -112,9 +129,9 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
   if (blockIdx.x == 0)
     for (uint32_t s = tid; s <= d.n_seqs; s += PT_THREADS) plan.prefix[s] = prefix[s];
   const uint64_t total = prefix[d.n_seqs] * d.n_kv_heads;
-  const uint32_t shares = pt_shares(total, plan.blocks);
-  if (blockIdx.x >= shares) return;
-  const uint64_t begin = pt_from(total, shares, blockIdx.x), end = pt_from(total, shares, blockIdx.x + 1);
+  const PtShares shares(total, plan.blocks);
+  if (blockIdx.x >= shares.n) return;
+  const uint64_t begin = shares.from(blockIdx.x), end = shares.from(blockIdx.x + 1);
   uint32_t s = 0;
   for (uint32_t hi = d.n_seqs; s + 1 < hi;) {  // the sequence that unit `begin` belongs to
     const uint32_t mid = (s + hi) / 2;
@@ -129,38 +146,42 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
     uint32_t first, n;
     pt_units(d, sq.len, sq.rows, first, n);
     const uint64_t local = x - prefix[s] * d.n_kv_heads;
-    const uint32_t chunks = chunks_of(sq.rows), item = (uint32_t)(local / n), ua = (uint32_t)(local % n), kvh = item / chunks, row_a = item % chunks * RI;
+    const uint32_t chunks = chunks_of(sq.rows), item = (uint32_t)pt_div(local, n), ua = (uint32_t)(local - (uint64_t)item * n), kvh = item / chunks, row_a = item % chunks * RI;
     const uint32_t ub = (uint32_t)min((uint64_t)n, ua + (end - x)), rows = min(RI, sq.rows * rep - row_a);
     const uint32_t *table = d.tables + sq.slot * d.ld_table;
-    const uint8_t *base = reinterpret_cast<const uint8_t *>(d.pages) + (uint64_t)kvh * (d.page_tokens / PG_UNIT) * UB;
-    // units of this warp: ua + warp, + 8, ...; the pages of 32 of them at a time are in the lanes
+    const uint8_t *base = reinterpret_cast<const uint8_t *>(d.pages) + (uint64_t)kvh * page_units * UB;
+    // steps of this warp: ua + warp, + 8, ...; the pages of 16 of them at a time are in the lanes, one for each unit
     const uint32_t mine = ub > ua + warp ? (ub - ua - warp + PT_WARPS - 1) / PT_WARPS : 0;
-    auto unit_at = [&](uint32_t i) { return first + ua + warp + PT_WARPS * i; };
-    uint32_t entry = 0;
-    auto look_up = [&](uint32_t i) {
-      entry = CUTB_NO_PAGE;
-      if (i + lane < mine) entry = __ldg(table + unit_at(i + lane) * PG_UNIT / d.page_tokens);
-    };
-    auto issue = [&](uint32_t i, uint32_t to) {  // every lane; pages that do not exist arrive without bytes
-      if (i % 32 == 0) look_up(i);
-      const uint32_t page = __shfl_sync(0xffffffffu, entry, i % 32);
-      if (lane == 0) {
-        if (page < d.n_pages) {
+    auto unit_at = [&](uint32_t i) { return 2 * (first + ua + warp + PT_WARPS * i); };
+    const uint8_t *source = nullptr;  // of this lane's unit
+    uint32_t pages_there = 0;         // of the 32 units
+    // Starts the copies of step i into stage `to`, each by the lane that has the unit's address; bit u of the result: unit u has
+    // keys and its page exists.
+    auto issue = [&](uint32_t i, uint32_t to) {
+      if (i % 16 == 0) {
+        const uint32_t k = i + lane / 2, unit = unit_at(k) + (lane & 1);
+        const bool keys = k < mine && unit * PG_UNIT < sq.len;
+        const uint32_t page = keys ? __ldg(table + (unit >> page_shift)) : CUTB_NO_PAGE;
+        if (keys && page >= d.n_pages) paged_report(d.status, CUTB_ERR_INVALID);
+        source = base + (uint64_t)page * d.page_bytes + (unit & page_mask) * UB;
+        pages_there = __ballot_sync(0xffffffffu, page < d.n_pages);
+      }
+      if (lane / 2 == i % 16) {
+        if (pages_there >> lane & 1) {
           mbar_arrive_expect_tx(bar + 8 * to, UB);
-          bulk_g2s(ring + to * UB, base + (uint64_t)page * d.page_bytes + unit_at(i) * PG_UNIT % d.page_tokens / PG_UNIT * UB, UB, bar + 8 * to);
+          bulk_g2s(ring + (to * 2 + (lane & 1)) * UB, source, UB, bar + 8 * to);
         } else {
           mbar_arrive(bar + 8 * to);
-          paged_report(d.status, CUTB_ERR_INVALID);
         }
       }
-      return page < d.n_pages;
+      return pages_there >> 2 * (i % 16) & 3u;
     };
-    uint32_t there = 0;  // bit of a stage: its page exists
+    uint32_t there = 0;  // two bits of each stage
     uint32_t issued = 0;
     if (!dead)
       for (; issued < min(mine, S); ++issued) {
         const uint32_t to = (stage + issued) % S;
-        there = issue(issued, to) ? there | 1u << to : there & ~(1u << to);
+        there = (there & ~(3u << 2 * to)) | issue(issued, to) << 2 * to;
       }
     // this lane's columns: query row of column g (fragments) and of columns 2 t, 2 t + 1 (scores)
     uint32_t qf[NT][2 * G][2];
@@ -174,18 +195,27 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
       const T *src = reinterpret_cast<const T *>(d.q) + (uint64_t)(sq.row0 + (live ? tok : 0)) * d.ldq + (uint64_t)(live ? hq : 0) * d.head_dim;
       float v[G][8], top = 0.f;
 #pragma unroll
-      for (int j = 0; j < G; ++j)
+      for (int j = 0; j < G; ++j) {
+        const uint32_t i = 32 * j + 8 * t;
+        if (plan.vec) {  // eight elements that are there or not
+          uint4 raw[sizeof(T) / 2] = {};
+          if (live && i < d.head_dim)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t i = 32 * j + 8 * t + e;
-          v[j][e] = live && i < d.head_dim ? to_f(src[i]) : 0.f;
-          top = fmaxf(top, fabsf(v[j][e]));
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) raw[k] = __ldg(reinterpret_cast<const uint4 *>(src + i) + k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = to_f(reinterpret_cast<const T *>(raw)[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = live && i + e < d.head_dim ? to_f(src[i + e]) : 0.f;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[j][e]));
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^-e of the largest element (of numbers too small or not finite: none)
       const uint32_t ex = __float_as_uint(top) >> 23;
-      const float down = ex > 0 && ex < 254 ? __uint_as_float((254 - ex) << 23) : 1.f, up = ex > 0 && ex < 254 ? __uint_as_float(ex << 23) : 1.f;
+      const float down = plan.sign * (ex > 0 && ex < 254 ? __uint_as_float((254 - ex) << 23) : 1.f), up = ex > 0 && ex < 254 ? __uint_as_float(ex << 23) : 1.f;
 #pragma unroll
       for (int j = 0; j < G; ++j)
 #pragma unroll
@@ -202,15 +232,17 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint32_t c = 2 * t + k, cr = SPLIT ? c & 3 : c, rr = row_a + nt * TILE + cr;
-        mult[nt][k] = __shfl_sync(0xffffffffu, up, cr * 4) * d.scale * 1.4426950408889634f;
+        mult[nt][k] = __shfl_sync(0xffffffffu, up, cr * 4) * plan.scale;
         at[nt][k] = cr < TILE && nt * TILE + cr < rows ? sq.len - sq.rows + rr / rep + 1 : 0;
       }
     }
     const uint32_t pos_min = sq.len - sq.rows + row_a / rep, pos_max = sq.len - sq.rows + (row_a + rows - 1) / rep;
-    float m[NT][2], l[NT][2], o[NT][MT][4];
+    // Weights are taken relative to `low`: 2^8 for a score that is the largest so far, up to 2^15 before `low` follows it, so that the
+    // values are rescaled rarely; fp16 pairs hold 2^-24 of that, and the sums are fp32 whatever their scale.
+    float low[NT][2], from[NT][2], l[NT][2], o[NT][MT][4];  // from: low where there is one
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+      low[nt][0] = low[nt][1] = -INFINITY, from[nt][0] = from[nt][1] = l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
@@ -220,14 +252,15 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
         dead = true;
         break;
       }
-      const uint8_t *u = pt_smem + (ring - smem_u32(pt_smem)) + stage * UB;
-      const bool exists = there >> stage & 1;
+      const uint8_t *u0 = pt_smem + (ring - smem_u32(pt_smem)) + stage * 2 * UB;
+      const uint32_t exists = there >> 2 * stage & 3;
       const uint32_t key0 = unit_at(i) * PG_UNIT;
-      const bool edge = !exists || key0 + PG_UNIT - 1 > pos_min || (d.window && pos_max >= key0 && pos_max - key0 >= d.window);
-      float sc[NT][4];
-      {
-        float acc[NT][2][4] = {};
-        uint32_t w0[G], w1[G], s0[G], s1[G];
+      const bool edge = exists != 3 || key0 + PT_KEYS - 1 > pos_min || (d.window && pos_max >= key0 && pos_max - key0 >= d.window);
+      float sc[NT][2][4] = {};  // (the two units' sums are independent chains)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t *u = u0 + half * UB;
+        alignas(16) uint32_t w0[G], w1[G], s0[G], s1[G];
         const uint32_t *k0 = reinterpret_cast<const uint32_t *>(u) + tk * (DP / 8), *k1 = k0 + 2 * (DP / 8);
         if constexpr (DP % 128 == 0) {
 #pragma unroll
@@ -243,10 +276,18 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
           }
         }
         const uint32_t *ks = reinterpret_cast<const uint32_t *>(u + pg_key_scales_at(DP)) + tk * G;
+        if constexpr (G % 4 == 0) {
 #pragma unroll
-        for (int j = 0; j < G; j += 2) {
-          *reinterpret_cast<uint2 *>(s0 + j) = *reinterpret_cast<const uint2 *>(ks + j);
-          *reinterpret_cast<uint2 *>(s1 + j) = *reinterpret_cast<const uint2 *>(ks + 2 * G + j);
+          for (int j = 0; j < G; j += 4) {
+            *reinterpret_cast<uint4 *>(s0 + j) = *reinterpret_cast<const uint4 *>(ks + j);
+            *reinterpret_cast<uint4 *>(s1 + j) = *reinterpret_cast<const uint4 *>(ks + 2 * G + j);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < G; j += 2) {
+            *reinterpret_cast<uint2 *>(s0 + j) = *reinterpret_cast<const uint2 *>(ks + j);
+            *reinterpret_cast<uint2 *>(s1 + j) = *reinterpret_cast<const uint2 *>(ks + 2 * G + j);
+          }
         }
 #pragma unroll
         for (int j = 0; j < G; ++j) {
@@ -258,94 +299,102 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
           for (int e = 0; e < 4; ++e) a[e] = __hfma2(a[e], d0, m0), b[e] = __hfma2(b[e], d1, m1);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(acc[nt][0], h2_as_u32(a[0]), h2_as_u32(b[0]), h2_as_u32(a[1]), h2_as_u32(b[1]), qf[nt][2 * j][0], qf[nt][2 * j][1]);
-            mma_f16(acc[nt][1], h2_as_u32(a[2]), h2_as_u32(b[2]), h2_as_u32(a[3]), h2_as_u32(b[3]), qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
+            mma_f16(sc[nt][half], h2_as_u32(a[0]), h2_as_u32(b[0]), h2_as_u32(a[1]), h2_as_u32(b[1]), qf[nt][2 * j][0], qf[nt][2 * j][1]);
+            mma_f16(sc[nt][half], h2_as_u32(a[2]), h2_as_u32(b[2]), h2_as_u32(a[3]), h2_as_u32(b[3]), qf[nt][2 * j + 1][0], qf[nt][2 * j + 1][1]);
           }
+        }
+        if (SPLIT)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sc[nt][half][c] += __shfl_xor_sync(0xffffffffu, sc[nt][half][c], 2);
+      }
+      if (edge) {
+        // what is past the sequence, or on a page that is not there, may be anything: its values become zeros
+        if (exists != 3 || key0 + PT_KEYS > sq.len) {
+          constexpr uint32_t WORDS = pg_unit_bytes(DP) / 10 / 4;  // of a unit's value scales, a word for two tokens
+          for (uint32_t e = lane; e < 2 * WORDS; e += 32) {
+            const uint32_t half = e / WORDS, w = e % WORDS, quad = w / 4 % 4, pair = w % 2;
+            uint32_t *to = reinterpret_cast<uint32_t *>(const_cast<uint8_t *>(u0) + half * UB + pg_value_scales_at(DP)) + w;
+            const uint32_t tok = key0 + half * PG_UNIT + 4 * quad + 2 * pair;
+            const uint32_t keep = !(exists >> half & 1) || tok >= sq.len ? 0u : tok + 1 >= sq.len ? 0xffffu : 0xffffffffu;
+            *to &= keep;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v = acc[nt][0][c] + acc[nt][1][c];
-            if (SPLIT) v += __shfl_xor_sync(0xffffffffu, v, 2);
-            sc[nt][c] = v * mult[nt][c & 1];
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t key = key0 + c / 4 * PG_UNIT + tk + (c & 2), p1 = at[nt][c & 1];
+            if (!(exists >> c / 4 & 1) || key >= p1 || (d.window && p1 - key > d.window)) sc[nt][c / 4][c % 4] = -INFINITY;
           }
       }
-      if (edge) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t key = key0 + tk + (c & 2), p1 = at[nt][c & 1];
-            if (!exists || key >= p1 || (d.window && p1 - key > d.window)) sc[nt][c] = -INFINITY;
-          }
-      }
-      uint32_t bf[NT][2];
+      uint32_t bf[NT][2][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float mx = fmaxf(sc[nt][k], sc[nt][k + 2]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(m[nt][k], mx);
-          f[k] = m[nt][k] == mn ? 1.f : pt_exp2(m[nt][k] - mn);
-          m[nt][k] = mn;
-        }
-        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
-          l[nt][0] *= f[0], l[nt][1] *= f[1];
+        for (int k = 0; k < 2; ++k) f[k] = fmaxf(fmaxf(sc[nt][0][k], sc[nt][0][k + 2]), fmaxf(sc[nt][1][k], sc[nt][1][k + 2]));
+        if (__any_sync(0xffffffffu, fmaf(f[0], mult[nt][0], -15.f) > low[nt][0] || fmaf(f[1], mult[nt][1], -15.f) > low[nt][1])) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float mx = f[k];
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float to = fmaxf(low[nt][k], fmaf(mx, mult[nt][k], -8.f));
+            f[k] = low[nt][k] == to ? 1.f : pt_exp2(low[nt][k] - to);
+            low[nt][k] = to, l[nt][k] *= f[k];
+            from[nt][k] = to == -INFINITY ? 0.f : to;
+          }
 #pragma unroll
           for (int i2 = 0; i2 < MT; ++i2) o[nt][i2][0] *= f[0], o[nt][i2][1] *= f[1], o[nt][i2][2] *= f[0], o[nt][i2][3] *= f[1];
         }
-        float p[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float mm = m[nt][c & 1];
-          p[c] = pt_exp2(sc[nt][c] - (mm == -INFINITY ? 0.f : mm - 15.f));
+        for (int half = 0; half < 2; ++half) {
+          float p[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) p[c] = pt_exp2(fmaf(sc[nt][half][c], mult[nt][c & 1], -from[nt][c & 1]));
+          l[nt][0] += p[0] + p[2], l[nt][1] += p[1] + p[3];
+          uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
+          if (SPLIT) {
+            const float2 a = __half22float2(u32_as_h2(h0)), b = __half22float2(u32_as_h2(h1));
+            const uint32_t l0 = pack_half(p[0] - a.x, p[1] - a.y), l1 = pack_half(p[2] - b.x, p[3] - b.y);
+            h0 = t < 2 ? h0 : l0, h1 = t < 2 ? h1 : l1;
+          }
+          bf[nt][half][0] = transposed(h0), bf[nt][half][1] = transposed(h1);
         }
-        l[nt][0] += p[0] + p[2], l[nt][1] += p[1] + p[3];
-        uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
-        if (SPLIT && t >= 2) {
-          const float2 a = __half22float2(u32_as_h2(h0)), b = __half22float2(u32_as_h2(h1));
-          h0 = pack_half(p[0] - a.x, p[1] - a.y), h1 = pack_half(p[2] - b.x, p[3] - b.y);
-        }
-        __syncwarp();
-        bf[nt][0] = transposed(h0), bf[nt][1] = transposed(h1);
       }
-      {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t *u = u0 + half * UB;
         const uint4 *vw = reinterpret_cast<const uint4 *>(u + pg_values_at(DP)) + lane;
         const uint4 *vs = reinterpret_cast<const uint4 *>(u + pg_value_scales_at(DP)) + t;
-        const bool tail = !exists || key0 + PG_UNIT > sq.len;  // what is past the sequence may be anything
 #pragma unroll
         for (int q4 = 0; q4 < MT / 4; ++q4) {
           const uint4 w = vw[32 * q4];
           const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint4 x = vs[4 * (2 * q4 + half)];
-            if (tail) {
-              const uint32_t left = !exists || sq.len <= key0 + 4 * t ? 0 : min(4u, sq.len - key0 - 4 * t);
-              const uint32_t m01 = left >= 2 ? 0xffffffffu : left ? 0xffffu : 0u, m23 = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
-              x.x &= m01, x.y &= m23, x.z &= m01, x.w &= m23;
-            }
+          for (int gr = 0; gr < 2; ++gr) {
+            const uint4 x = vs[4 * (2 * q4 + gr)];
             const __half2 dA = u32_as_h2(x.x), dB = u32_as_h2(x.y), mA = u32_as_h2(x.z), mB = u32_as_h2(x.w);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               __half2 a[4];
-              pg_quants(ws[2 * half + k], a);
+              pg_quants(ws[2 * gr + k], a);
               a[0] = __hfma2(a[0], dA, mA), a[1] = __hfma2(a[1], dA, mA), a[2] = __hfma2(a[2], dB, mB), a[3] = __hfma2(a[3], dB, mB);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma_f16(o[nt][4 * q4 + 2 * half + k], h2_as_u32(a[0]), h2_as_u32(a[1]), h2_as_u32(a[2]), h2_as_u32(a[3]), bf[nt][0], bf[nt][1]);
+                mma_f16(o[nt][4 * q4 + 2 * gr + k], h2_as_u32(a[0]), h2_as_u32(a[1]), h2_as_u32(a[2]), h2_as_u32(a[3]), bf[nt][half][0], bf[nt][half][1]);
             }
           }
         }
       }
-      __syncwarp();  // the unit is read
+      __syncwarp();  // the units are read
       if (issued < mine) {
-        there = issue(issued, stage) ? there | 1u << stage : there & ~(1u << stage);
+        there = (there & ~(3u << 2 * stage)) | issue(issued, stage) << 2 * stage;
         ++issued;
       }
       if (++stage == S) stage = 0, phase ^= 1u;
@@ -354,26 +403,18 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
       for (uint32_t i = 0; i < S; ++i) mbar_drain(bar + 8 * i, i < stage ? phase ^ 1u : phase);  // nothing may land in a block that has ended
       if (lane == 0) paged_report(d.status, CUTB_ERR_TIMEOUT);
     }
-    // the warps' parts meet: maxima and sums, then the values under the common maximum
+    // the warps' parts meet, each in its warp's ring; the low parts of fp32 rows join their high parts
+    float *vals = reinterpret_cast<float *>(pt_smem + warp * S * 2 * UB);  // [row][LD]
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float v = l[nt][k];
         v += __shfl_xor_sync(0xffffffffu, v, 4), v += __shfl_xor_sync(0xffffffffu, v, 8), v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (g == 0) m_s[warp][8 * nt + 2 * t + k] = m[nt][k], l_s[warp][8 * nt + 2 * t + k] = v;
+        if (g == 0) part_s[8 * nt + 2 * t + k][warp] = make_float2(low[nt][k], v);
       }
-    __syncthreads();  // (and every warp is done with its ring)
-    float *vals = reinterpret_cast<float *>(pt_smem);  // [warp][row][LD]; the low parts of fp32 rows join their high parts
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float f[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float top = -INFINITY;
-        for (uint32_t w = 0; w < PT_WARPS; ++w) top = fmaxf(top, m_s[w][8 * nt + 2 * t + k]);
-        f[k] = m[nt][k] == -INFINITY ? 0.f : pt_exp2(m[nt][k] - top);
-      }
+      const bool in0 = nt * TILE + 2 * t < rows, in1 = nt * TILE + 2 * t + 1 < rows;
+      float *to = vals + (nt * TILE + 2 * t) * LD + g;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         float y[4];
@@ -381,25 +422,28 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
         for (int c = 0; c < 4; ++c) {
           y[c] = o[nt][i][c];
           if (SPLIT) y[c] += __shfl_xor_sync(0xffffffffu, y[c], 2);
-          y[c] *= f[c & 1];
         }
         if (!SPLIT || t < 2) {
-          float *to = vals + (warp * RI + nt * TILE + 2 * t) * LD + 16 * i + g;
-          to[0] = y[0], to[LD] = y[1], to[8] = y[2], to[LD + 8] = y[3];
+          if (in0) to[16 * i] = y[0], to[16 * i + 8] = y[2];
+          if (in1) to[16 * i + LD] = y[1], to[16 * i + LD + 8] = y[3];
         }
       }
     }
     __syncthreads();
     const bool whole = ua == 0 && ub == n;
     float *part = plan.part + ((uint64_t)blockIdx.x * 2 + (ua == 0)) * RI * (DP + 2);
-    for (uint32_t e = tid; e < RI * DP; e += PT_THREADS) {
+    for (uint32_t e = tid; e < rows * DP; e += PT_THREADS) {
       const uint32_t r = e / DP, i = e % DP, c = r / TILE * 8 + r % TILE;
-      if (r >= rows) break;
+      float2 w[PT_WARPS];
       float y = 0.f, top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (uint32_t w = 0; w < PT_WARPS; ++w) y += vals[(w * RI + r) * LD + i], top = fmaxf(top, m_s[w][c]);
+      for (uint32_t k = 0; k < PT_WARPS; ++k) w[k] = part_s[c][k], top = fmaxf(top, w[k].x);
 #pragma unroll
-      for (uint32_t w = 0; w < PT_WARPS; ++w) sum += m_s[w][c] == -INFINITY ? 0.f : l_s[w][c] * pt_exp2(m_s[w][c] - top);
+      for (uint32_t k = 0; k < PT_WARPS; ++k) {
+        const float f = w[k].x == -INFINITY ? 0.f : pt_exp2(w[k].x - top);
+        sum = fmaf(f, w[k].y, sum);
+        y = fmaf(f, reinterpret_cast<const float *>(pt_smem + k * S * 2 * UB)[r * LD + i], y);
+      }
       if (whole) {
         const uint32_t rr = row_a + r;
         if (i < d.head_dim)
@@ -415,36 +459,55 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
   }
 }
 
-// Joins the parts of the KV heads' units that several blocks worked on, in the order of the units.
-template <typename T> __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ cutb_paged_desc d, const PtPlan plan) {
+// Joins the parts of the KV heads' steps that several blocks worked on, in the order of the steps: a block per query row, which
+// weighs all parts first.
+constexpr uint32_t PJ_THREADS = 128;
+template <typename T> __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_constant__ cutb_paged_desc d, const PtPlan plan) {
+  extern __shared__ float2 weight_s[];  // of part b: {largest score, sum}, then its weight
+  __shared__ float warps[2][4];
   pdl_enter();
-  const uint32_t of = gridDim.x / d.n_seqs, s = blockIdx.x / of, kvh = blockIdx.y, chunk = blockIdx.x % of, dp = pg_pad(d.head_dim), rep = d.n_heads / d.n_kv_heads, RI = plan.rows;
+  const uint32_t RI = plan.rows, of = gridDim.x / d.n_seqs, s = blockIdx.x / of, kvh = blockIdx.y, row = blockIdx.x % of;
+  const uint32_t dp = pg_pad(d.head_dim), rep = d.n_heads / d.n_kv_heads, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(d, s);
-  const uint32_t chunks = (sq.rows * rep + RI - 1) / RI;
-  if (chunk >= chunks) return;
+  if (row >= sq.rows * rep) return;
+  const uint32_t chunks = (sq.rows * rep + RI - 1) / RI, chunk = row / RI, r = row % RI;
   const uint64_t total = plan.prefix[d.n_seqs] * d.n_kv_heads;
   uint32_t first, n;
   pt_units(d, sq.len, sq.rows, first, n);
   const uint64_t a = plan.prefix[s] * d.n_kv_heads + (uint64_t)(kvh * chunks + chunk) * n;
-  const uint32_t shares = pt_shares(total, plan.blocks);
-  auto block_of = [&](uint64_t x) {
-    uint32_t b = (uint32_t)(x * shares / total);
-    while (pt_from(total, shares, b + 1) <= x) ++b;
-    return b;
-  };
-  const uint32_t b0 = block_of(a), b1 = block_of(a + n - 1);
-  if (b0 == b1) return;
-  const uint32_t row_a = chunk * RI, rows = min(RI, sq.rows * rep - row_a);
-  auto part = [&](uint32_t b, uint32_t r) { return plan.part + (((uint64_t)b * 2 + (b == b0)) * RI + r) * (dp + 2); };
-  for (uint32_t e = threadIdx.x; e < rows * d.head_dim; e += 128) {
-    const uint32_t r = e / d.head_dim, i = e % d.head_dim, rr = row_a + r;
-    float top = -INFINITY, y = 0.f, sum = 0.f;
-    for (uint32_t b = b0; b <= b1; ++b) top = fmaxf(top, part(b, r)[dp]);
-    for (uint32_t b = b0; b <= b1; ++b) {
-      const float *p = part(b, r), f = p[dp] == -INFINITY ? 0.f : pt_exp2(p[dp] - top);
-      y = fmaf(f, p[i], y), sum = fmaf(f, p[dp + 1], sum);
-    }
-    reinterpret_cast<T *>(d.out)[(uint64_t)(sq.row0 + rr / rep) * d.ldo + (uint64_t)(kvh * rep + rr % rep) * d.head_dim + i] = from_f<T>(sum > 0.f ? y / sum : 0.f);
+  const PtShares shares(total, plan.blocks);
+  const uint32_t b0 = shares.block_of(a), parts = shares.block_of(a + n - 1) - b0 + 1;
+  if (parts == 1) return;
+  const uint64_t step = 2ull * RI * (dp + 2);
+  const float *mid = plan.part + (uint64_t)b0 * step + (uint64_t)r * (dp + 2);  // of block b0 + k: k steps on; the first has its second slot
+  auto part = [&](uint32_t k) { return mid + k * step + (k ? 0 : (uint64_t)RI * (dp + 2)); };
+  float top = -INFINITY;
+  for (uint32_t k = tid; k < parts; k += PJ_THREADS) {
+    weight_s[k] = make_float2(part(k)[dp], part(k)[dp + 1]);
+    top = fmaxf(top, weight_s[k].x);
+  }
+#pragma unroll
+  for (int o = 16; o; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) warps[0][tid / 32] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(warps[0][0], warps[0][1]), fmaxf(warps[0][2], warps[0][3]));
+  float sum = 0.f;
+  for (uint32_t k = tid; k < parts; k += PJ_THREADS) {
+    const float2 w = weight_s[k];
+    const float f = w.x == -INFINITY ? 0.f : pt_exp2(w.x - top);
+    weight_s[k].x = f, sum = fmaf(f, w.y, sum);
+  }
+#pragma unroll
+  for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((tid & 31) == 0) warps[1][tid / 32] = sum;
+  __syncthreads();
+  sum = (warps[1][0] + warps[1][1]) + (warps[1][2] + warps[1][3]);
+  T *out = reinterpret_cast<T *>(d.out) + (uint64_t)(sq.row0 + row / rep) * d.ldo + (uint64_t)(kvh * rep + row % rep) * d.head_dim;
+  for (uint32_t i = tid; i < d.head_dim; i += PJ_THREADS) {
+    float y = 0.f;
+#pragma unroll 8
+    for (uint32_t k = 0; k < parts; ++k) y = fmaf(weight_s[k].x, part(k)[i], y);
+    out[i] = from_f<T>(sum > 0.f ? y / sum : 0.f);
   }
 }
 
@@ -460,6 +523,8 @@ int pt_plan(const cutb_paged_desc &d, PtPlan *p, uint64_t *bytes) {
   const uint32_t nt = pt_tiles(d), dp = pg_pad(d.head_dim);
   p->rows = (d.dtype == CUTB_F32 ? 4 : 8) * nt;
   p->blocks = di.sm_count * (dp * nt <= 128 ? 2 : 1);
+  p->scale = d.scale == 0.f ? 1.f : fabsf(d.scale) * 1.4426950408889634f, p->sign = d.scale == 0.f ? 0.f : d.scale < 0.f ? -1.f : 1.f;
+  p->vec = d.head_dim % 8 == 0 && d.ldq * (d.dtype == CUTB_F32 ? 4 : 2) % 16 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
   const uint64_t prefix = (8ull * (d.n_seqs + 1) + 255) / 256 * 256;
   p->prefix = reinterpret_cast<uint64_t *>(d.workspace);
   p->part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(d.workspace) + prefix);
@@ -470,11 +535,11 @@ int pt_plan(const cutb_paged_desc &d, PtPlan *p, uint64_t *bytes) {
 template <typename T, int DP, int NT> int pt_launch(const cutb_paged_desc &d, const PtPlan &p, cudaStream_t stream) {
   const uint32_t smem = pt_ring_bytes(DP) + 8 * (d.n_seqs + 1) + (uint32_t)sizeof(PtSeq) * d.n_seqs;
   const uint32_t most = pt_ring_bytes(DP) + 8 * (PG_MAX_SEQS + 1) + (uint32_t)sizeof(PtSeq) * PG_MAX_SEQS;
-  static_assert(PT_WARPS * (sizeof(T) == 4 ? 4 : 8) * NT * (DP + 4) * 4 <= pt_ring_bytes(DP), "the parts meet in the rings");
+  static_assert((sizeof(T) == 4 ? 4 : 8) * NT * (DP + 4) * 4 <= pt_ring_bytes(DP) / PT_WARPS, "a warp's part fits in its ring");
   CUTB_CUDA_TRY(cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
   CUTB_CUDA_TRY(launch_pdl(paged_attention_kernel<T, DP, NT>, dim3(p.blocks), dim3(PT_THREADS), smem, stream, d, p));
-  const uint32_t chunks = (uint32_t)(((uint64_t)(d.max_new < d.n_tokens ? d.max_new : d.n_tokens) * (d.n_heads / d.n_kv_heads) + p.rows - 1) / p.rows);
-  CUTB_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3(d.n_seqs * chunks, d.n_kv_heads), dim3(128), 0, stream, d, p));
+  const uint32_t rows = (d.max_new < d.n_tokens ? d.max_new : d.n_tokens) * (d.n_heads / d.n_kv_heads);
+  CUTB_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3(d.n_seqs * rows, d.n_kv_heads), dim3(PJ_THREADS), 8 * p.blocks, stream, d, p));
   return CUTB_OK;
 }
 

@@ -76,13 +76,18 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 
 // Eight nibbles of a word as four pairs of the fp16 numbers d q + m: bits of q under the exponent of 1024 are 1024 + q (or 1024 + 16 q),
 // from which q comes back exactly; the last step rounds once.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {  // a & b | c, one instruction
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 __device__ __forceinline__ void pg_quants(uint32_t w, __half2 (&q)[4]) {
   const __half2 k1024 = u32_as_h2(0x64006400u), k16th = u32_as_h2(0x2c002c00u), k64 = u32_as_h2(0xd400d400u);  // 1024, 1 / 16, -64
   const uint32_t v = w >> 8;
-  q[0] = __hsub2(u32_as_h2((w & 0x000f000fu) | 0x64006400u), k1024);
-  q[1] = __hfma2(u32_as_h2((w & 0x00f000f0u) | 0x64006400u), k16th, k64);
-  q[2] = __hsub2(u32_as_h2((v & 0x000f000fu) | 0x64006400u), k1024);
-  q[3] = __hfma2(u32_as_h2((v & 0x00f000f0u) | 0x64006400u), k16th, k64);
+  q[0] = __hsub2(u32_as_h2(and_or(w, 0x000f000fu, 0x64006400u)), k1024);
+  q[1] = __hfma2(u32_as_h2(and_or(w, 0x00f000f0u, 0x64006400u)), k16th, k64);
+  q[2] = __hsub2(u32_as_h2(and_or(v, 0x000f000fu, 0x64006400u)), k1024);
+  q[3] = __hfma2(u32_as_h2(and_or(v, 0x00f000f0u, 0x64006400u)), k16th, k64);
 }
 
 #endif  // __CUDACC__
