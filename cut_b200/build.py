@@ -18,7 +18,7 @@ LAYER_SOURCES = ["cabi_layers.cu", "common.cu", "layer_ops.cu", "mixer_ops.cu", 
                  "latent_attention.cu", "moe.cu", "expert_matvec.cu", "sample.cu"]
 QUANT_SOURCES = ["cabi.cu", "qgemv_blocks.cu", "qgemv_row.cu", "qgemv_few.cu", "qgemm_few.cu", "qgemm_wide.cu", "qmatmul_generic.cu", "dequant.cu", "transpose_q4.cu",
                  "qgemm_tc.cu", "qgemm_skinny.cu", "repack.cu", "attention.cu", "attention_prefill.cu", "qgemv_planes.cu", "qgemv_rows.cu",
-                 "cabi_paged.cu", "paged_cache.cu", "paged_attention.cu"]
+                 "cabi_paged.cu", "paged_cache.cu", "paged_attention.cu", "paged_prefill.cu"]
 SOURCES = QUANT_SOURCES + LAYER_SOURCES
 LAYERS_LIB = os.path.join(HERE, "libcutb_layers.so")
 HEADERS = ["common.cuh", "matvec_common.cuh", "tmem_weights.cuh", "kernels.h", "tcgen05.cuh", "qgemm_tc_common.cuh", "dense_common.cuh", "norm_stage.cuh",

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint32_t c = 2 * t + k, cr = SPLIT ? c & 3 : c, rr = row_a + nt * TILE + cr;
-        mult[nt][k] = __shfl_sync(0xffffffffu, up, cr * 4) * plan.scale;
+        mult[nt][k] = fmaxf(__shfl_sync(0xffffffffu, up, cr * 4) * plan.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
         at[nt][k] = cr < TILE && nt * TILE + cr < rows ? sq.len - sq.rows + rr / rep + 1 : 0;
       }
     }
@@ -546,12 +546,14 @@ template <typename T, int DP, int NT> int pt_launch(const cutb_paged_desc &d, co
 }  // namespace
 
 uint64_t paged_attention_workspace(const cutb_paged_desc &d) {
+  if (paged_prefill_applies(d)) return 0;
   PtPlan p;
   uint64_t bytes = 0;
   return pt_plan(d, &p, &bytes) == CUTB_OK ? bytes : 0;
 }
 
 int paged_attention_launch(const cutb_paged_desc &d, cudaStream_t stream) {
+  if (paged_prefill_applies(d)) return paged_prefill_launch(d, stream);
   PtPlan p;
   uint64_t bytes;
   if (int rc = pt_plan(d, &p, &bytes)) return rc;
