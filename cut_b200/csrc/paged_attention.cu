@@ -368,27 +368,37 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
         }
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint8_t *u = u0 + half * UB;
-        const uint4 *vw = reinterpret_cast<const uint4 *>(u + pg_values_at(DP)) + lane;
-        const uint4 *vs = reinterpret_cast<const uint4 *>(u + pg_value_scales_at(DP)) + t;
+      for (int q4 = 0; q4 < MT / 4; ++q4) {
+        uint4 w4[2];
 #pragma unroll
-        for (int q4 = 0; q4 < MT / 4; ++q4) {
-          const uint4 w = vw[32 * q4];
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        for (int half = 0; half < 2; ++half) w4[half] = *(reinterpret_cast<const uint4 *>(u0 + half * UB + pg_values_at(DP)) + 32 * q4 + lane);
 #pragma unroll
-          for (int gr = 0; gr < 2; ++gr) {
-            const uint4 x = vs[4 * (2 * q4 + gr)];
-            const __half2 dA = u32_as_h2(x.x), dB = u32_as_h2(x.y), mA = u32_as_h2(x.z), mB = u32_as_h2(x.w);
+        for (int gr = 0; gr < 2; ++gr) {
+          uint4 x[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+          for (int half = 0; half < 2; ++half) x[half] = *(reinterpret_cast<const uint4 *>(u0 + half * UB + pg_value_scales_at(DP)) + 4 * (2 * q4 + gr) + t);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            // fp32 rows: a step's values are added here, rounded; tensor cores cut off what a long sum cannot hold
+            float fresh[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) fresh[nt][c] = SPLIT ? 0.f : o[nt][4 * q4 + 2 * gr + k][c];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const __half2 dA = u32_as_h2(x[half].x), dB = u32_as_h2(x[half].y), mA = u32_as_h2(x[half].z), mB = u32_as_h2(x[half].w);
+              const uint32_t ws[4] = {w4[half].x, w4[half].y, w4[half].z, w4[half].w};
               __half2 a[4];
               pg_quants(ws[2 * gr + k], a);
               a[0] = __hfma2(a[0], dA, mA), a[1] = __hfma2(a[1], dA, mA), a[2] = __hfma2(a[2], dB, mB), a[3] = __hfma2(a[3], dB, mB);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma_f16(o[nt][4 * q4 + 2 * gr + k], h2_as_u32(a[0]), h2_as_u32(a[1]), h2_as_u32(a[2]), h2_as_u32(a[3]), bf[nt][half][0], bf[nt][half][1]);
+              for (int nt = 0; nt < NT; ++nt) mma_f16(fresh[nt], h2_as_u32(a[0]), h2_as_u32(a[1]), h2_as_u32(a[2]), h2_as_u32(a[3]), bf[nt][half][0], bf[nt][half][1]);
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][4 * q4 + 2 * gr + k][c] = SPLIT ? o[nt][4 * q4 + 2 * gr + k][c] + fresh[nt][c] : fresh[nt][c];
           }
         }
       }

@@ -25,10 +25,11 @@ constexpr uint32_t PP_KEYS = 128, PP_UNPACK = 8, PP_PLANE = 128 * 128;  // bytes
 template <typename T, int DP> struct PpShape {
   static constexpr bool SPLIT = sizeof(T) == 4;
   static constexpr uint32_t X = SPLIT || DP > 128 ? 1 : 2, TERMS = SPLIT ? 2 : 1;
-  static constexpr uint32_t SK = DP <= 128 || (DP == 192 && !SPLIT) ? 2 : 1, SV = DP <= 128 ? 2 : 1;
+  static constexpr uint32_t SK = DP <= 192 ? 2 : 1, SV = DP <= 128 ? 2 : 1;
   static constexpr uint32_t QT = DP / 64 * PP_PLANE, KT = QT, VT = DP * 256;  // bytes of a tile
   static constexpr uint32_t SMEM = 1024 + X * TERMS * QT + SK * KT + SV * VT, WARPS = 4 * X + 1 + PP_UNPACK;
-  static constexpr uint32_t LOW = 128, OUT = 256;  // tensor memory columns: scores and weights from 0, low parts (X = 1), values
+  // tensor memory columns: scores and weights from 0, low parts (X = 1), values, and (SPLIT) the values of the tiles before
+  static constexpr uint32_t LOW = 128, OUT = 256, TOTAL = 384;
 };
 
 struct PpParams {
@@ -44,6 +45,14 @@ __device__ __forceinline__ float pp_exp2(float x) {
 __device__ __forceinline__ uint32_t pp_pack(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
 __device__ __forceinline__ uint32_t pp_sw(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 __device__ __forceinline__ uint32_t pp_fma(__half2 q, __half2 d, __half2 m) { return h2_as_u32(__hfma2(q, d, m)); }
+__device__ __forceinline__ void pp_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void pp_sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -249,7 +258,8 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
 #pragma unroll
           for (uint32_t ks = 0; ks < DP / 16; ++ks) {
             const uint32_t off = (ks >> 2) * (PP_PLANE >> 4) + (ks & 3) * 2;
-            umma_f16(tmem + x * 128, q_lo + (x * S::TERMS + term) * (QT >> 4) + off, k_lo + sk * (KT >> 4) + off, desc_hi, id_s, term | ks ? 1u : 0u);
+            // (low parts first, while the sum is small: tensor cores cut off what a sum cannot hold)
+            umma_f16(tmem + x * 128, q_lo + (x * S::TERMS + S::TERMS - 1 - term) * (QT >> 4) + off, k_lo + sk * (KT >> 4) + off, desc_hi, id_s, term | ks ? 1u : 0u);
           }
         umma_commit(sfull + x * 8);
       }
@@ -266,7 +276,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
           for (uint32_t term = 0; term < S::TERMS; ++term)
 #pragma unroll
             for (uint32_t ks = 4 * half; ks < 4 * half + 4; ++ks)
-              umma_ts(tmem + S::OUT + x * DP, tmem + (term ? S::LOW : x * 128) + ks * 8, v_lo + sv * (VT >> 4) + (ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2, desc_hi, id_o,
+              umma_ts(tmem + S::OUT + x * DP, tmem + (term + 1 < S::TERMS ? S::LOW : x * 128) + ks * 8, v_lo + sv * (VT >> 4) + (ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2, desc_hi, id_o,
                       term | ks ? 1u : acc[x]);
         }
       }
@@ -275,7 +285,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         umma_commit(odone + x * 8);
         if (last) umma_commit(vempty + sv * 8);
       }
-      acc[x] = 1;
+      acc[x] = SPLIT ? 0 : 1;
       if (last && ++sv == SV) sv = 0, pv ^= 1u;
     };
     bool pending = false;  // the second row tile's value product over the tile before
@@ -355,7 +365,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       __syncwarp();
       if (lane == 0) mbar_arrive(qready);
     }
-    const uint32_t mine = tmem + ((warp & 3) << 21), s_t = mine + x * 128, l_t = mine + S::LOW, o_t = mine + S::OUT + x * DP;
+    const uint32_t mine = tmem + ((warp & 3) << 21), s_t = mine + x * 128, l_t = mine + S::LOW, o_t = mine + S::OUT + x * DP, t_t = mine + S::TOTAL;
     float low = -INFINITY, from = 0.f, l = 0.f;
     uint32_t ph = 0, done = 0;
     bool dead = false;
@@ -393,25 +403,38 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         for (uint32_t i = 0; i < 32; ++i) m4[i % 4] = fmaxf(m4[i % 4], __uint_as_float(s[i]));
         mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
       }
-      if (__any_sync(0xffffffffu, fmaf(mx, mult, -15.f) > low)) {
-        const float to = fmaxf(low, fmaf(mx, mult, -8.f)), f = low == to ? 1.f : pp_exp2(low - to);
+      const bool rises = __any_sync(0xffffffffu, fmaf(mx, mult, -15.f) > low);
+      float f = 1.f;
+      if (rises) {
+        const float to = fmaxf(low, fmaf(mx, mult, -8.f));
+        f = low == to ? 1.f : pp_exp2(low - to);
         low = to, l *= f, from = to == -INFINITY ? 0.f : to;
-        if (done) {
-          if (!warp_wait(odone + x * 8, (done - 1) & 1u)) {
-            dead = true;
-            break;
-          }
-          tc_fence_after();
-#pragma unroll 1
-          for (uint32_t c = 0; c < DP; c += 32) {
-            uint32_t o[32], a[16], b[16];
-            tmem_ld32(o_t + c, o);
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) a[i] = __float_as_uint(__uint_as_float(o[i]) * f), b[i] = __float_as_uint(__uint_as_float(o[16 + i]) * f);
-            tmem_st16(o_t + c, a);
-            tmem_st16(o_t + c + 16, b);
-          }
+      }
+      // The weighted values follow.  Those of fp32 rows leave the tensor cores after every tile and are added here: a sum that goes on
+      // there loses half a unit of its last place at every product of 16 keys.
+      if (done && (rises || SPLIT)) {
+        if (!warp_wait(odone + x * 8, (done - 1) & 1u)) {
+          dead = true;
+          break;
         }
+        tc_fence_after();
+#pragma unroll 1
+        for (uint32_t c = 0; c < DP; c += 16) {
+          uint32_t o[16];
+          pp_ld16(o_t + c, o);
+          if constexpr (SPLIT) {
+            if (done > 1) {
+              uint32_t y[16];
+              pp_ld16(t_t + c, y);
+#pragma unroll
+              for (uint32_t i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(y[i]));
+            }
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st16(SPLIT ? t_t + c : o_t + c, o);
+        }
+        if constexpr (SPLIT) tmem_wait_st();
       }
 #pragma unroll 1
       for (uint32_t j = 0; j < 4; ++j) {
@@ -458,6 +481,14 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         uint32_t o[32];
         __syncwarp();
         tmem_ld32(o_t + c, o);
+        if constexpr (SPLIT) {
+          if (done > 1) {
+            uint32_t y[32];
+            tmem_ld32(t_t + c, y);
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(y[i]));
+          }
+        }
         if (!live) continue;
         if (pp.out_vec) {
           constexpr uint32_t N = 16 / sizeof(T);
@@ -502,8 +533,8 @@ template <typename T, int DP> int pp_launch(const cutb_paged_desc &d, cudaStream
 }  // namespace
 
 bool paged_prefill_applies(const cutb_paged_desc &d) {
-  // (two terms of 256 elements do not fit in shared memory beside a tile of keys and one of values)
-  if (d.dtype == CUTB_F32 && pg_pad(d.head_dim) == 256) return false;
+  // (tensor memory does not hold the values of an fp32 tile of wider heads twice, beside its scores)
+  if (d.dtype == CUTB_F32 && pg_pad(d.head_dim) > 128) return false;
   return (uint64_t)d.max_new * (d.n_heads / d.n_kv_heads) > 32;
 }
 
@@ -513,9 +544,8 @@ int paged_prefill_launch(const cutb_paged_desc &d, cudaStream_t stream) {
     switch (pg_pad(d.head_dim)) {
       case 64: return pp_launch<T, 64>(d, stream);
       case 128: return pp_launch<T, 128>(d, stream);
-      case 192: return pp_launch<T, 192>(d, stream);
       default:
-        if constexpr (sizeof(T) == 2) return pp_launch<T, 256>(d, stream);
+        if constexpr (sizeof(T) == 2) return pg_pad(d.head_dim) == 192 ? pp_launch<T, 192>(d, stream) : pp_launch<T, 256>(d, stream);
         else return (int)CUTB_ERR_UNSUPPORTED;
     }
   });
