@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
       if (i % 16 == 0) {
         const uint32_t k = i + lane / 2, unit = unit_at(k) + (lane & 1);
         const bool keys = k < mine && unit * PG_UNIT < sq.len;
-        const uint32_t page = keys ? __ldg(table + (unit >> page_shift)) : CUTB_NO_PAGE;
+        const uint32_t page = keys ? table[unit >> page_shift] : CUTB_NO_PAGE;
         if (keys && page >= d.n_pages) paged_report(d.status, CUTB_ERR_INVALID);
         source = base + (uint64_t)page * d.page_bytes + (unit & page_mask) * UB;
         pages_there = __ballot_sync(0xffffffffu, page < d.n_pages);
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
     }
     const uint32_t tk = 4 * (g / 2) + (g & 1);  // the token of MMA row g; row g + 8 is the second after it
     for (uint32_t i = 0; i < mine && !dead; ++i) {
-      if (!warp_wait(bar + 8 * stage, phase)) {
+      if (!warp_wait_one(bar + 8 * stage, phase)) {
         dead = true;
         break;
       }

@@ -79,7 +79,7 @@ template <typename T> __global__ void __launch_bounds__(256) paged_kv_write_kern
   const uint32_t pos = sq.len - sq.rows + (row - sq.row0), dp = pg_pad(d.head_dim);
   uint32_t page = 0;
   if (!bad) {
-    page = __ldg(d.tables + sq.slot * d.ld_table + pos / d.page_tokens);
+    page = d.tables[sq.slot * d.ld_table + pos / d.page_tokens];
     bad = page >= d.n_pages || (d.rot_dims && pos >= d.max_pos);
   }
   if (bad) {
@@ -163,7 +163,7 @@ template <typename T> __global__ void __launch_bounds__(256) paged_kv_read_kerne
   const PagedSeq sq = paged_seq(d, s);
   if (!sq.bad && row - sq.row0 >= sq.rows) return;
   const uint32_t pos = sq.len - sq.rows + (row - sq.row0), dp = pg_pad(d.head_dim), t = pos % PG_UNIT, groups = dp / 32;
-  const uint32_t page = sq.bad ? CUTB_NO_PAGE : __ldg(d.tables + sq.slot * d.ld_table + pos / d.page_tokens);
+  const uint32_t page = sq.bad ? CUTB_NO_PAGE : d.tables[sq.slot * d.ld_table + pos / d.page_tokens];
   if (page >= d.n_pages) {
     if (lane == 0) paged_report(d.status, CUTB_ERR_INVALID);
     return;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(PB_THREADS) pages_reserve_kernel(const __grid_
   const PagesPlan plan = pages_plan(d.workspace, d.n_pages);
   const uint32_t i = threadIdx.x, lane = i & 31, P = d.page_tokens;
   const bool mine = i < d.n;
-  const uint32_t s = mine ? __ldg(d.items + i) : 0, grow = mine ? __ldg(d.counts + i) : 0;
+  const uint32_t s = mine ? d.items[i] : 0, grow = mine ? d.counts[i] : 0;
   slot_s[i] = mine ? s : 0xffffffffu;
   __syncthreads();
   bool ok = mine && s < d.n_slots;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(PB_THREADS) pages_fork_kernel(const __grid_con
   pdl_enter();
   const uint32_t i = threadIdx.x, lane = i & 31;
   const bool mine = i < d.n;
-  const uint32_t src = mine ? __ldg(d.items + i) : 0, dst = mine ? __ldg(d.others + i) : 0;
+  const uint32_t src = mine ? d.items[i] : 0, dst = mine ? d.others[i] : 0;
   dst_s[i] = mine ? dst : 0xffffffffu, src_s[i] = src;
   __syncthreads();
   bool ok = mine && src < d.n_slots && dst < d.n_slots && src != dst;
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(PB_THREADS) pages_free_kernel(const __grid_con
   pdl_enter();
   const uint32_t i = threadIdx.x, lane = i & 31;
   const bool mine = i < d.n;
-  const uint32_t s = mine ? __ldg(d.items + i) : 0;
+  const uint32_t s = mine ? d.items[i] : 0;
   uint32_t n = 0;
   if (mine && s >= d.n_slots) paged_report(d.status, CUTB_ERR_INVALID);
   if (mine && s < d.n_slots) {

@@ -39,12 +39,12 @@ struct PagedSeq {
 };
 __device__ __forceinline__ PagedSeq paged_seq(const cutb_paged_desc &d, uint32_t s) {
   PagedSeq q;
-  q.row0 = d.starts ? __ldg(d.starts + s) : s;
-  const uint32_t end = d.starts ? __ldg(d.starts + s + 1) : s + 1;
-  q.slot = d.slots ? __ldg(d.slots + s) : s;
+  q.row0 = d.starts ? d.starts[s] : s;
+  const uint32_t end = d.starts ? d.starts[s + 1] : s + 1;
+  q.slot = d.slots ? d.slots[s] : s;
   q.bad = end < q.row0 || end > d.n_tokens || end - q.row0 > d.max_new || q.slot >= d.n_slots;
   q.rows = q.bad ? 0 : end - q.row0;
-  q.len = q.slot < d.n_slots ? __ldg(d.lengths + q.slot) : 0;
+  q.len = q.slot < d.n_slots ? d.lengths[q.slot] : 0;
   if (q.rows && (q.len < q.rows || q.len > d.ld_table * d.page_tokens)) q.bad = true, q.rows = 0;
   return q;
 }
@@ -58,13 +58,23 @@ __device__ __forceinline__ uint32_t paged_seq_of(const cutb_paged_desc &d, uint3
   uint32_t lo = 0, hi = d.n_seqs;
   for (;;) {  // 32 places at a time
     const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const uint32_t n = __popc(__ballot_sync(0xffffffffu, at < hi && __ldg(d.starts + min(at, hi - 1)) <= row));
+    const uint32_t n = __popc(__ballot_sync(0xffffffffu, at < hi && d.starts[min(at, hi - 1)] <= row));
     if (n == 0) return d.n_seqs;
     lo += (n - 1) * step, hi = min(lo + step, hi);
     if (step == 1) return lo;
   }
 }
 
+// A wait of a whole warp by one of its lanes.  (32 lanes that ask for one barrier queue up at the shared-memory pipe, which shuffles and
+// loads of the other warps need as well: with a whole warp spinning, 40 shuffles of another one took 13000 cycles.) 
+__device__ __forceinline__ bool warp_wait_one(uint32_t bar, uint32_t parity) {
+  bool ok = false;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait_probe_first(bar, parity);
+  ok = __any_sync(0xffffffffu, ok);
+  __syncwarp();
+  return ok;
+}
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f(float v) { return v; }
 template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }

@@ -7,7 +7,7 @@
 //                   rows, weights are relative to a reference that follows the maximum in steps of 2^7, so that the weighted values are rarely
 //                   rescaled; what the scores lack to the reference is exact.
 //   issuing warp    scores = Q K^T from shared memory, weighted values = P (tensor memory) V; fp32 rows with two terms of Q and of P
-//   unpacking warps (8) a unit of 16 tokens each: nibbles from global memory (the next tile's are on their way while this one's are
+//   unpacking warps (7; 16 warps have 128 registers a thread) take turns over units of 16 tokens: nibbles from global memory (the next tile's are on their way while this one's are
 //                   turned into fp16), written as the tensor cores read them: K with a token to a row, V with an element to a row, as
 //                   its units keep four neighbouring tokens together; 128-byte swizzle.
 // A tile of 128 keys costs 256 rows of 128 elements about 2000 cycles of tensor cores, as many of exponentials, and the unpacking 800
@@ -20,7 +20,7 @@
 namespace cutb {
 namespace {
 
-constexpr uint32_t PP_KEYS = 128, PP_UNPACK = 8, PP_PLANE = 128 * 128;  // bytes of 64 columns of 128 rows
+constexpr uint32_t PP_KEYS = 128, PP_UNITS = 8, PP_UNPACK = 7, PP_PLANE = 128 * 128;  // bytes of 64 columns of 128 rows
 
 template <typename T, int DP> struct PpShape {
   static constexpr bool SPLIT = sizeof(T) == 4;
@@ -45,13 +45,24 @@ __device__ __forceinline__ float pp_exp2(float x) {
 __device__ __forceinline__ uint32_t pp_pack(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
 __device__ __forceinline__ uint32_t pp_sw(uint32_t row, uint32_t chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 __device__ __forceinline__ uint32_t pp_fma(__half2 q, __half2 d, __half2 m) { return h2_as_u32(__hfma2(q, d, m)); }
+// Tensor memory into registers, the wait in the same statement: the loads write their registers whenever they come, and a copy of one that
+// the compiler puts between two statements would read what was there before and free the register for something else.
+__device__ __forceinline__ void pp_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void pp_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                  "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(taddr)
                : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void pp_sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -67,27 +78,32 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   constexpr uint32_t X = S::X, SK = S::SK, SV = S::SV, QT = S::QT, KT = S::KT, VT = S::VT, G = DP / 32, UB = pg_unit_bytes(DP), ROWS = X * 128;
   extern __shared__ __align__(1024) uint8_t pp_raw[];
   const uint32_t smem = (smem_u32(pp_raw) + 1023) & ~1023u, q_u = smem, k_u = q_u + X * S::TERMS * QT, v_u = k_u + SK * KT;
-  __shared__ __align__(8) uint64_t bars[2 * SK + 2 * SV + 4 * X + 1];
+  __shared__ __align__(8) uint64_t bars[2 * SK + 2 * SV + 4 * X + 2];
   __shared__ uint32_t tmem_slot, abort_flag, bad_s, seq_s, tile_s;
+  __shared__ float mult_s[ROWS];
+  __shared__ PagedSeq found_s;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t kfull = smem_u32(bars), kempty = kfull + SK * 8, vfull = kempty + SK * 8, vempty = vfull + SV * 8;
-  const uint32_t sfull = vempty + SV * 8, pready = sfull + X * 8, odone = pready + 2 * X * 8, qready = odone + X * 8;
+  const uint32_t sfull = vempty + SV * 8, pready = sfull + X * 8, odone = pready + 2 * X * 8, qready = odone + X * 8, drained = qready + 8;
   if (tid == 0) {
-    for (uint32_t i = 0; i < SK; ++i) mbar_init(kfull + i * 8, PP_UNPACK), mbar_init(kempty + i * 8, 1);
-    for (uint32_t i = 0; i < SV; ++i) mbar_init(vfull + i * 8, PP_UNPACK), mbar_init(vempty + i * 8, 1);
+    for (uint32_t i = 0; i < SK; ++i) mbar_init(kfull + i * 8, PP_UNITS), mbar_init(kempty + i * 8, 1);
+    for (uint32_t i = 0; i < SV; ++i) mbar_init(vfull + i * 8, PP_UNITS), mbar_init(vempty + i * 8, 1);
     for (uint32_t x = 0; x < X; ++x) mbar_init(sfull + x * 8, 1), mbar_init(odone + x * 8, 1), mbar_init(pready + 2 * x * 8, 4), mbar_init(pready + (2 * x + 1) * 8, 4);
-    mbar_init(qready, 4 * X);
-    abort_flag = 0, bad_s = 0, seq_s = d.n_seqs;
+    mbar_init(qready, 4 * X), mbar_init(drained, 1);
+    abort_flag = 0, bad_s = 0;
     fence_mbar_init();
   }
   pdl_enter();
   const uint32_t rep = d.n_heads / d.n_kv_heads, kvh = blockIdx.y;
   if (warp == 4 * X) {  // the sequence and the row tile that the block works on: 32 sequences at a time
     uint32_t before = 0;
+    if (lane == 0) seq_s = d.n_seqs;
+    __syncwarp();
     for (uint32_t s0 = 0; s0 < d.n_seqs; s0 += 32) {
       uint32_t tiles = 0;
+      PagedSeq q = {};
       if (s0 + lane < d.n_seqs) {
-        const PagedSeq q = paged_seq(d, s0 + lane);
+        q = paged_seq(d, s0 + lane);
         if (q.bad && blockIdx.x == 0 && kvh == 0) paged_report(d.status, CUTB_ERR_INVALID);
         tiles = (q.rows * rep + ROWS - 1) / ROWS;
       }
@@ -98,7 +114,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         if (lane >= o) sum += y;
       }
       const uint32_t mine = before + sum - tiles;
-      if (blockIdx.x >= mine && blockIdx.x < mine + tiles) seq_s = s0 + lane, tile_s = tiles - 1 - (blockIdx.x - mine);  // the later tokens (more keys) first
+      if (blockIdx.x >= mine && blockIdx.x < mine + tiles) seq_s = s0 + lane, found_s = q, tile_s = tiles - 1 - (blockIdx.x - mine);  // the later tokens (more keys) first
       before += __shfl_sync(0xffffffffu, sum, 31);
       if (blockIdx.x < before && blockIdx.x) break;  // (block 0 looks at all of them)
     }
@@ -106,9 +122,16 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   }
   __syncthreads();
   if (seq_s >= d.n_seqs) return;
-  const PagedSeq sq = paged_seq(d, seq_s);
+  const PagedSeq sq = found_s;
+  // (what every address below is made of, once more)
+  if (sq.slot >= d.n_slots || sq.rows == 0 || sq.rows > d.n_tokens || sq.row0 > d.n_tokens - sq.rows || sq.len < sq.rows || sq.len > d.ld_table * d.page_tokens ||
+      tile_s >= (sq.rows * rep + ROWS - 1) / ROWS) {
+    if (tid == 0) paged_report(d.status, CUTB_ERR_INVALID);
+    return;
+  }
   const uint32_t row_a = tile_s * ROWS, n_rows = min(ROWS, sq.rows * rep - row_a), pos0 = sq.len - sq.rows;
   if (warp == 4 * X) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -125,7 +148,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   const uint32_t *table = d.tables + sq.slot * d.ld_table;
   const uint32_t page_units = d.page_tokens / PG_UNIT, page_mask = page_units - 1, page_shift = 31 - __clz(page_units);
   for (uint32_t p = t_first * 8 / page_units + tid; p <= (key_hi - 1) / d.page_tokens; p += S::WARPS * 32)
-    if (__ldg(table + p) >= d.n_pages) bad_s = 1;
+    if (table[p] >= d.n_pages) bad_s = 1;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -140,24 +163,25 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   auto aborted = [&]() { return *reinterpret_cast<volatile uint32_t *>(&abort_flag) != 0; };
 
   if (warp > 4 * X) {
-    // ---- unpacking: unit dw of every tile ----
+    // ---- unpacking: the warps take turns over the units of all tiles ----
     constexpr uint32_t KQ = DP / 64;  // 16-byte pieces of a unit's keys, and of its values, in a lane
-    const uint32_t dw = warp - 4 * X - 1, r = lane / 4, quad = lane % 4;
+    const uint32_t r = lane / 4, quad = lane % 4, n_end = 8 * t_end;
     const uint8_t *base = reinterpret_cast<const uint8_t *>(d.pages) + (uint64_t)kvh * page_units * UB;
     uint4 kw[KQ], vw[KQ], vs[G];
     uint32_t ks[KQ][G];
     bool there_k = false, there_v = false;
     auto token_of = [&](uint32_t k) { return (128 * k + 4 * lane) / (DP / 8); };  // (a piece lies within one token)
-    auto unit_of = [&](uint32_t t, const uint8_t *&u) {
-      const uint32_t unit = 8 * t + dw;
+    auto unit_of = [&](uint32_t unit, const uint8_t *&u) {
+      u = base;
       if (unit * PG_UNIT >= sq.len) return false;
-      const uint32_t page = __ldg(table + (unit >> page_shift));
+      const uint32_t page = table[unit >> page_shift];
+      if (page >= d.n_pages) return false;
       u = base + (uint64_t)page * d.page_bytes + (unit & page_mask) * UB;
-      return page < d.n_pages;
+      return true;
     };
-    auto load_keys = [&](uint32_t t) {
+    auto load_keys = [&](uint32_t unit) {
       const uint8_t *u;
-      if (!(there_k = unit_of(t, u))) return;
+      if (!(there_k = unit_of(unit, u))) return;
 #pragma unroll
       for (uint32_t k = 0; k < KQ; ++k) {
         kw[k] = __ldg(reinterpret_cast<const uint4 *>(u) + 32 * k + lane);
@@ -166,19 +190,21 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         for (uint32_t j = 0; j < G; j += 2) *reinterpret_cast<uint2 *>(&ks[k][j]) = __ldg(reinterpret_cast<const uint2 *>(sc + j));
       }
     };
-    auto load_values = [&](uint32_t t) {
+    auto load_values = [&](uint32_t unit) {
       const uint8_t *u;
-      if (!(there_v = unit_of(t, u))) return;
+      if (!(there_v = unit_of(unit, u))) return;
 #pragma unroll
       for (uint32_t k = 0; k < KQ; ++k) vw[k] = __ldg(reinterpret_cast<const uint4 *>(u + pg_values_at(DP)) + 32 * k + lane);
 #pragma unroll
       for (uint32_t j = 0; j < G; ++j) vs[j] = __ldg(reinterpret_cast<const uint4 *>(u + pg_value_scales_at(DP)) + 4 * j + quad);
     };
-    load_keys(t_first);
-    load_values(t_first);
-    uint32_t sk = 0, pk = 1, sv = 0, pv = 1;  // (a fresh barrier lets a wait on the phase before its first pass)
-    for (uint32_t t = t_first; t < t_end; ++t) {
-      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(kempty + sk * 8, pk) && !aborted())) {
+    uint32_t unit = 8 * t_first + warp - 4 * X - 1;
+    load_keys(unit);
+    load_values(unit);
+    for (; unit < n_end; unit += PP_UNPACK) {
+      // (a fresh barrier lets a wait on the phase before its first pass)
+      const uint32_t i0 = unit / 8 - t_first, dw = unit % 8, sk = i0 % SK, pk = ~(i0 / SK) & 1, sv = i0 % SV, pv = ~(i0 / SV) & 1, next = unit + PP_UNPACK;
+      if (!warp_wait_one(kempty + sk * 8, pk) || __any_sync(0xffffffffu, aborted())) {
         if (lane == 0) give_up();
         break;
       }
@@ -212,14 +238,13 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(kfull + sk * 8);
-      if (++sk == SK) sk = 0, pk ^= 1u;
-      if (t + 1 < t_end) load_keys(t + 1);
-      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(vempty + sv * 8, pv) && !aborted())) {
+      if (next < n_end) load_keys(next);
+      if (!warp_wait_one(vempty + sv * 8, pv) || __any_sync(0xffffffffu, aborted())) {
         if (lane == 0) give_up();
         break;
       }
       {
-        const uint32_t tok0 = (8 * t + dw) * PG_UNIT + 4 * quad, left = !there_v || tok0 >= sq.len ? 0 : min(4u, sq.len - tok0);
+        const uint32_t tok0 = unit * PG_UNIT + 4 * quad, left = !there_v || tok0 >= sq.len ? 0 : min(4u, sq.len - tok0);
         const uint32_t m01 = left >= 2 ? 0xffffffffu : left ? 0xffffu : 0u, m23 = left >= 4 ? 0xffffffffu : left == 3 ? 0xffffu : 0u;
         const uint32_t dst = v_u + sv * VT + dw / 4 * (DP * 128) + (quad & 1) * 8, chunk = dw % 4 * 2 + quad / 2;
 #pragma unroll
@@ -237,22 +262,22 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(vfull + sv * 8);
-      if (++sv == SV) sv = 0, pv ^= 1u;
-      if (t + 1 < t_end) load_values(t + 1);
+      if (next < n_end) load_values(next);
     }
     __syncwarp();
   } else if (warp == 4 * X) {
-    // ---- products ----
+    // ---- products: one lane waits and issues ----
+    // (the other lanes have nothing to do: where they voted on every wait, a commit between two waits was carried out twice)
     const bool leader = elect_one();
-    const uint64_t proto = umma_desc_sw128(0);
-    const uint32_t desc_hi = (uint32_t)(proto >> 32), q_lo = (uint32_t)proto + ((q_u & 0x3FFFFu) >> 4), k_lo = (uint32_t)proto + ((k_u & 0x3FFFFu) >> 4);
-    const uint32_t v_lo = (uint32_t)proto + ((v_u & 0x3FFFFu) >> 4);
-    constexpr uint32_t id_s = umma_idesc_f16(128, 128), id_o = umma_idesc_f16(128, DP);
-    uint32_t sk = 0, pk = 0, sv = 0, pv = 0, pp_[2] = {0, 0}, acc[2] = {0, 0};
-    bool ok = __all_sync(0xffffffffu, mbar_spin_bounded(qready, 0));
-    tc_fence_after();
-    auto scores = [&](uint32_t x) {
-      if (leader) {
+    if (leader) {
+      const uint64_t proto = umma_desc_sw128(0);
+      const uint32_t desc_hi = (uint32_t)(proto >> 32), q_lo = (uint32_t)proto + ((q_u & 0x3FFFFu) >> 4), k_lo = (uint32_t)proto + ((k_u & 0x3FFFFu) >> 4);
+      const uint32_t v_lo = (uint32_t)proto + ((v_u & 0x3FFFFu) >> 4);
+      constexpr uint32_t id_s = umma_idesc_f16(128, 128), id_o = umma_idesc_f16(128, DP);
+      uint32_t sk = 0, pk = 0, sv = 0, pv = 0, pp_[2] = {0, 0}, acc[2] = {0, 0};
+      bool ok = mbar_spin_bounded(qready, 0);
+      tc_fence_after();
+      auto scores = [&](uint32_t x) {
 #pragma unroll
         for (uint32_t term = 0; term < S::TERMS; ++term)
 #pragma unroll
@@ -262,16 +287,14 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
             umma_f16(tmem + x * 128, q_lo + (x * S::TERMS + S::TERMS - 1 - term) * (QT >> 4) + off, k_lo + sk * (KT >> 4) + off, desc_hi, id_s, term | ks ? 1u : 0u);
           }
         umma_commit(sfull + x * 8);
-      }
-    };
-    auto values = [&](uint32_t x, bool last) {
-      ok = ok && __all_sync(0xffffffffu, mbar_spin_bounded(vfull + sv * 8, pv));
+      };
+      auto values = [&](uint32_t x, bool last) {
+        ok = ok && mbar_spin_bounded(vfull + sv * 8, pv);
 #pragma unroll
-      for (uint32_t half = 0; half < 2; ++half) {
-        ok = ok && __all_sync(0xffffffffu, mbar_spin_bounded(pready + (2 * x + half) * 8, pp_[x]));
-        if (!ok) return;
-        tc_fence_after();
-        if (leader) {
+        for (uint32_t half = 0; half < 2; ++half) {
+          ok = ok && mbar_spin_bounded(pready + (2 * x + half) * 8, pp_[x]);
+          if (!ok) return;
+          tc_fence_after();
 #pragma unroll
           for (uint32_t term = 0; term < S::TERMS; ++term)
 #pragma unroll
@@ -279,37 +302,38 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
               umma_ts(tmem + S::OUT + x * DP, tmem + (term + 1 < S::TERMS ? S::LOW : x * 128) + ks * 8, v_lo + sv * (VT >> 4) + (ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2, desc_hi, id_o,
                       term | ks ? 1u : acc[x]);
         }
-      }
-      pp_[x] ^= 1u;
-      if (leader) {
+        pp_[x] ^= 1u;
         umma_commit(odone + x * 8);
         if (last) umma_commit(vempty + sv * 8);
+        acc[x] = SPLIT ? 0 : 1;
+        if (last && ++sv == SV) sv = 0, pv ^= 1u;
+      };
+      bool pending = false;  // the second row tile's value product over the tile before
+      for (uint32_t t = t_first; t < t_end && ok; ++t) {
+        const bool s0 = sees(0, t), s1 = X > 1 && sees(1, t);
+        ok = mbar_spin_bounded(kfull + sk * 8, pk);
+        if (!ok) break;
+        tc_fence_after();
+        if (s0) {
+          scores(0);
+          if (!s1) umma_commit(kempty + sk * 8);
+        }
+        if (pending) values(1, true);
+        pending = s1;
+        if (!ok) break;
+        if (s1) {
+          scores(1);
+          umma_commit(kempty + sk * 8);
+        }
+        if (s0) values(0, !s1);
+        if (++sk == SK) sk = 0, pk ^= 1u;
       }
-      acc[x] = SPLIT ? 0 : 1;
-      if (last && ++sv == SV) sv = 0, pv ^= 1u;
-    };
-    bool pending = false;  // the second row tile's value product over the tile before
-    for (uint32_t t = t_first; t < t_end && ok; ++t) {
-      const bool s0 = sees(0, t), s1 = X > 1 && sees(1, t);
-      ok = __all_sync(0xffffffffu, mbar_spin_bounded(kfull + sk * 8, pk));
-      if (!ok) break;
-      tc_fence_after();
-      if (s0) {
-        scores(0);
-        if (!s1 && leader) umma_commit(kempty + sk * 8);
-      }
-      if (pending) values(1, true);
-      pending = s1;
-      if (!ok) break;
-      if (s1) {
-        scores(1);
-        if (leader) umma_commit(kempty + sk * 8);
-      }
-      if (s0) values(0, !s1);
-      if (++sk == SK) sk = 0, pk ^= 1u;
+      if (ok && pending) values(1, true);
+      if (!ok) give_up();
+      // products in flight read this block's shared memory and write its tensor memory: they end before it does, whoever gave up
+      umma_commit(drained);
+      if (!mbar_test(drained, 0)) (void)mbar_wait_bounded(drained, 0, 1u << 10);
     }
-    if (ok && pending) values(1, true);
-    if (!ok && leader) give_up();
     __syncwarp();
   } else {
     // ---- a row's queries, scaled by a power of two, as one or two fp16 terms; then its softmax ----
@@ -317,54 +341,69 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     const bool live = x * 128 + row < n_rows;
     const uint32_t pos = pos0 + Rc / rep;
     const uint64_t token = sq.row0 + Rc / rep, head = (uint64_t)(kvh * rep + Rc % rep) * d.head_dim;
-    float mult;
     {
-      const T *src = reinterpret_cast<const T *>(d.q) + token * d.ldq + head;
-      auto eight = [&](uint32_t i, float (&v)[8]) {  // elements i .. i + 7 of the row
-        if (pp.vec) {
-          uint4 raw[sizeof(T) / 2] = {};
-          if (i < d.head_dim)
+      // a warp takes every 4 X-th row, its lanes neighbouring elements of it, eight rows at a time
+      constexpr uint32_t E = DP / 32, W4 = E * sizeof(T) / 4, BATCH = 8;  // elements and words of a lane
+#pragma unroll 1
+      for (uint32_t r0 = warp; r0 < ROWS; r0 += 4 * X * BATCH) {
+        uint32_t raw[BATCH][W4];
 #pragma unroll
-            for (uint32_t k = 0; k < sizeof(T) / 2; ++k) raw[k] = __ldg(reinterpret_cast<const uint4 *>(src + i) + k);
+        for (uint32_t k = 0; k < BATCH; ++k) {
+          const uint32_t r = r0 + 4 * X * k, Rr = row_a + min(r, n_rows - 1);
+          const T *src = reinterpret_cast<const T *>(d.q) + (uint64_t)(sq.row0 + Rr / rep) * d.ldq + (uint64_t)(kvh * rep + Rr % rep) * d.head_dim + E * lane;
+          if (pp.vec) {  // (a lane's elements are there or not)
+            if constexpr (W4 == 4) {
+              *reinterpret_cast<uint4 *>(raw[k]) = E * lane < d.head_dim ? __ldg(reinterpret_cast<const uint4 *>(src)) : make_uint4(0, 0, 0, 0);
+            } else if constexpr (W4 == 2) {
+              *reinterpret_cast<uint2 *>(raw[k]) = E * lane < d.head_dim ? __ldg(reinterpret_cast<const uint2 *>(src)) : make_uint2(0, 0);
+            } else {
 #pragma unroll
-          for (uint32_t e = 0; e < 8; ++e) v[e] = to_f(reinterpret_cast<const T *>(raw)[e]);
-        } else {
+              for (uint32_t i = 0; i < W4; ++i) raw[k][i] = E * lane + i * 4 / sizeof(T) < d.head_dim ? __ldg(reinterpret_cast<const uint32_t *>(src) + i) : 0u;
+            }
+          } else {
+            T *e = reinterpret_cast<T *>(raw[k]);
 #pragma unroll
-          for (uint32_t e = 0; e < 8; ++e) v[e] = i + e < d.head_dim ? to_f(src[i + e]) : 0.f;
-        }
-      };
-      float top = 0.f, v[8];
-#pragma unroll 4
-      for (uint32_t c = 0; c < DP / 8; ++c) {
-        eight(8 * c, v);
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-      }
-      const uint32_t ex = __float_as_uint(top) >> 23;
-      const bool fits = ex > 0 && ex < 254;
-      const float down = (live ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : 1.f);
-      mult = fmaxf((fits ? __uint_as_float(ex << 23) : 1.f) * pp.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
-#pragma unroll 4
-      for (uint32_t c = 0; c < DP / 8; ++c) {
-        eight(8 * c, v);
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          const float a = v[2 * e] * down, b = v[2 * e + 1] * down;
-          h[e] = pp_pack(a, b);
-          if constexpr (SPLIT) {
-            const float2 f = __half22float2(u32_as_h2(h[e]));
-            l[e] = pp_pack(a - f.x, b - f.y);
+            for (uint32_t i = 0; i < E; ++i) e[i] = E * lane + i < d.head_dim ? src[i] : from_f<T>(0.f);
           }
         }
-        const uint32_t at = q_u + x * S::TERMS * QT + c / 8 * PP_PLANE + pp_sw(row, c % 8);
-        pp_sts16(at, h[0], h[1], h[2], h[3]);
-        if constexpr (SPLIT) pp_sts16(at + QT, l[0], l[1], l[2], l[3]);
+        float top[BATCH];
+#pragma unroll
+        for (uint32_t k = 0; k < BATCH; ++k) {
+          const T *e = reinterpret_cast<const T *>(raw[k]);
+          top[k] = 0.f;
+#pragma unroll
+          for (uint32_t i = 0; i < E; ++i) top[k] = fmaxf(top[k], fabsf(to_f(e[i])));
+        }
+#pragma unroll
+        for (int o = 16; o; o /= 2)
+#pragma unroll
+          for (uint32_t k = 0; k < BATCH; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+#pragma unroll
+        for (uint32_t k = 0; k < BATCH; ++k) {
+          const T *e = reinterpret_cast<const T *>(raw[k]);
+          const uint32_t r = r0 + 4 * X * k, ex = __float_as_uint(top[k]) >> 23;
+          const bool fits = ex > 0 && ex < 254;
+          const float down = (r < n_rows ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : 1.f);
+          if (lane == 0) mult_s[r] = fmaxf((fits ? __uint_as_float(ex << 23) : 1.f) * pp.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
+#pragma unroll
+          for (uint32_t i = 0; i < E; i += 2) {
+            const float f0 = to_f(e[i]) * down, f1 = to_f(e[i + 1]) * down;
+            const uint32_t h = pp_pack(f0, f1), c = E * lane + i;
+            const uint32_t at = q_u + (r >> 7) * S::TERMS * QT + c / 64 * PP_PLANE + pp_sw(r & 127, c % 64 / 8) + c % 8 * 2;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(h) : "memory");
+            if constexpr (SPLIT) {
+              const float2 f = __half22float2(u32_as_h2(h));
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + QT), "r"(pp_pack(f0 - f.x, f1 - f.y)) : "memory");
+            }
+          }
+        }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(qready);
+      asm volatile("bar.sync 1, %0;" ::"n"(4 * X * 32) : "memory");
     }
+    const float mult = mult_s[x * 128 + row];
     const uint32_t mine = tmem + ((warp & 3) << 21), s_t = mine + x * 128, l_t = mine + S::LOW, o_t = mine + S::OUT + x * DP, t_t = mine + S::TOTAL;
     float low = -INFINITY, from = 0.f, l = 0.f;
     uint32_t ph = 0, done = 0;
@@ -373,7 +412,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     for (uint32_t t = t_first; t < t_end; ++t) {
       const uint32_t key0 = t * PP_KEYS;
       if (!(key0 < my_hi && key0 + PP_KEYS > my_lo)) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(sfull + x * 8, ph) && !aborted())) {
+      if (!warp_wait_one(sfull + x * 8, ph) || __any_sync(0xffffffffu, aborted())) {
         dead = true;
         break;
       }
@@ -384,7 +423,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       uint32_t gone = 0;  // units on pages that do not exist
       if (any_bad)
         for (uint32_t u = 0; u < 8; ++u)
-          if ((8 * t + u) * PG_UNIT < my_hi && __ldg(table + ((8 * t + u) >> page_shift)) >= d.n_pages) gone |= 1u << u;
+          if ((8 * t + u) * PG_UNIT < my_hi && table[(8 * t + u) >> page_shift] >= d.n_pages) gone |= 1u << u;
       auto masked = [&](uint32_t j, uint32_t (&s)[32]) {
 #pragma unroll
         for (uint32_t i = 0; i < 32; ++i) {
@@ -396,7 +435,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
 #pragma unroll 1
       for (uint32_t j = 0; j < 4; ++j) {
         uint32_t s[32];
-        tmem_ld32(s_t + 32 * j, s);
+        pp_ld32(s_t + 32 * j, s);
         if (!all) masked(j, s);
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -413,7 +452,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       // The weighted values follow.  Those of fp32 rows leave the tensor cores after every tile and are added here: a sum that goes on
       // there loses half a unit of its last place at every product of 16 keys.
       if (done && (rises || SPLIT)) {
-        if (!warp_wait(odone + x * 8, (done - 1) & 1u)) {
+        if (!warp_wait_one(odone + x * 8, (done - 1) & 1u)) {
           dead = true;
           break;
         }
@@ -439,7 +478,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
 #pragma unroll 1
       for (uint32_t j = 0; j < 4; ++j) {
         uint32_t s[32], h[16];
-        tmem_ld32(s_t + 32 * j, s);
+        pp_ld32(s_t + 32 * j, s);
         if (!all) masked(j, s);
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
@@ -463,12 +502,12 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(pready + (2 * x + (j >> 1)) * 8);
+          if (lane == 0) mbar_arrive(pready + (2 * x + j / 2) * 8);
         }
       }
       ++done;
     }
-    if (!dead && done && !warp_wait(odone + x * 8, (done - 1) & 1u)) dead = true;
+    if (!dead && done && !warp_wait_one(odone + x * 8, (done - 1) & 1u)) dead = true;
     if (dead) {
       if (lane == 0) give_up();
     } else if (done) {
@@ -480,11 +519,11 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         if (c >= d.head_dim) break;
         uint32_t o[32];
         __syncwarp();
-        tmem_ld32(o_t + c, o);
+        pp_ld32(o_t + c, o);
         if constexpr (SPLIT) {
           if (done > 1) {
             uint32_t y[32];
-            tmem_ld32(t_t + c, y);
+            pp_ld32(t_t + c, y);
 #pragma unroll
             for (uint32_t i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(y[i]));
           }
