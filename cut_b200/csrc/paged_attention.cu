@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
   __shared__ __align__(8) uint64_t bars[PT_WARPS * S];
   __shared__ __align__(16) float2 part_s[8 * NT][PT_WARPS];  // of a column and a warp: what its weights are relative to, their sum
   __shared__ uint64_t sums[PT_WARPS], carry_s;
-  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane / 4, t = lane % 4;
+  const uint32_t tid = threadIdx.x, warp = warp_index(), lane = tid & 31, g = lane / 4, t = lane % 4;
   const uint32_t bar = smem_u32(bars) + warp * S * 8, ring = smem_u32(pt_smem) + warp * S * 2 * UB;
   const uint32_t page_units = d.page_tokens / PG_UNIT, page_mask = page_units - 1, page_shift = 31 - __clz(page_units);
   if (lane == 0) {

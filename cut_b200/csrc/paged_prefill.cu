@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   __shared__ uint32_t tmem_slot, abort_flag, bad_s, seq_s, tile_s;
   __shared__ float mult_s[ROWS];
   __shared__ PagedSeq found_s;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
   const uint32_t kfull = smem_u32(bars), kempty = kfull + SK * 8, vfull = kempty + SK * 8, vempty = vfull + SV * 8;
   const uint32_t sfull = vempty + SV * 8, pready = sfull + X * 8, odone = pready + 2 * X * 8, qready = odone + X * 8, drained = qready + 8;
   if (tid == 0) {
@@ -342,54 +342,66 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     const uint32_t pos = pos0 + Rc / rep;
     const uint64_t token = sq.row0 + Rc / rep, head = (uint64_t)(kvh * rep + Rc % rep) * d.head_dim;
     {
-      // a warp takes every 4 X-th row, its lanes neighbouring elements of it, eight rows at a time
-      constexpr uint32_t E = DP / 32, W4 = E * sizeof(T) / 4, BATCH = 8;  // elements and words of a lane
+      // The rows come as they are to the bytes that their terms will have (asynchronous copies, all at once); then a warp turns 32
+      // rows of its own into terms.  Little code: straight-line code is fetched once per block, a few hundred cycles a line.
+      constexpr uint32_t PIECES = DP * sizeof(T) / 16, E = DP / 32;  // 16-byte pieces of a row, elements of a lane
+      auto place = [&](uint32_t r, uint32_t byte) {  // of a raw row's byte
+        return q_u + (r >> 7) * S::TERMS * QT + byte / 128 * PP_PLANE + (r & 127) * 128 + byte % 128;
+      };
+      const uint32_t r0 = warp * 32;
 #pragma unroll 1
-      for (uint32_t r0 = warp; r0 < ROWS; r0 += 4 * X * BATCH) {
-        uint32_t raw[BATCH][W4];
+      for (uint32_t i = lane; i < 32 * PIECES; i += 32) {
+        const uint32_t r = r0 + i / PIECES, c = i % PIECES, Rr = row_a + min(r, n_rows - 1), e = c * 16 / sizeof(T);
+        const T *src = reinterpret_cast<const T *>(d.q) + (uint64_t)(sq.row0 + Rr / rep) * d.ldq + (uint64_t)(kvh * rep + Rr % rep) * d.head_dim + e;
+        const uint32_t dst = place(r, c * 16);
+        if (pp.vec && e < d.head_dim) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        } else {
+          T raw[16 / sizeof(T)];
 #pragma unroll
-        for (uint32_t k = 0; k < BATCH; ++k) {
-          const uint32_t r = r0 + 4 * X * k, Rr = row_a + min(r, n_rows - 1);
-          const T *src = reinterpret_cast<const T *>(d.q) + (uint64_t)(sq.row0 + Rr / rep) * d.ldq + (uint64_t)(kvh * rep + Rr % rep) * d.head_dim + E * lane;
-          if (pp.vec) {  // (a lane's elements are there or not)
-            if constexpr (W4 == 4) {
-              *reinterpret_cast<uint4 *>(raw[k]) = E * lane < d.head_dim ? __ldg(reinterpret_cast<const uint4 *>(src)) : make_uint4(0, 0, 0, 0);
-            } else if constexpr (W4 == 2) {
-              *reinterpret_cast<uint2 *>(raw[k]) = E * lane < d.head_dim ? __ldg(reinterpret_cast<const uint2 *>(src)) : make_uint2(0, 0);
-            } else {
-#pragma unroll
-              for (uint32_t i = 0; i < W4; ++i) raw[k][i] = E * lane + i * 4 / sizeof(T) < d.head_dim ? __ldg(reinterpret_cast<const uint32_t *>(src) + i) : 0u;
-            }
-          } else {
-            T *e = reinterpret_cast<T *>(raw[k]);
-#pragma unroll
-            for (uint32_t i = 0; i < E; ++i) e[i] = E * lane + i < d.head_dim ? src[i] : from_f<T>(0.f);
-          }
+          for (uint32_t k = 0; k < 16 / sizeof(T); ++k) raw[k] = e + k < d.head_dim ? src[k] : from_f<T>(0.f);
+          const uint4 w = *reinterpret_cast<const uint4 *>(raw);
+          pp_sts16(dst, w.x, w.y, w.z, w.w);
         }
-        float top[BATCH];
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      constexpr uint32_t B = 4;  // rows at a time
+#pragma unroll 1
+      for (uint32_t r = r0; r < r0 + 32; r += B) {
+        float v[B][E], top[B];
 #pragma unroll
-        for (uint32_t k = 0; k < BATCH; ++k) {
-          const T *e = reinterpret_cast<const T *>(raw[k]);
+        for (uint32_t k = 0; k < B; ++k) {
           top[k] = 0.f;
 #pragma unroll
-          for (uint32_t i = 0; i < E; ++i) top[k] = fmaxf(top[k], fabsf(to_f(e[i])));
+          for (uint32_t i = 0; i < E; i += 2) {
+            const uint32_t at = place(r + k, (E * lane + i) * sizeof(T));
+            if constexpr (SPLIT) {
+              asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[k][i]), "=f"(v[k][i + 1]) : "r"(at) : "memory");
+            } else {
+              uint32_t w;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+              const T *e = reinterpret_cast<const T *>(&w);
+              v[k][i] = to_f(e[0]), v[k][i + 1] = to_f(e[1]);
+            }
+            top[k] = fmaxf(top[k], fmaxf(fabsf(v[k][i]), fabsf(v[k][i + 1])));
+          }
         }
 #pragma unroll
         for (int o = 16; o; o /= 2)
 #pragma unroll
-          for (uint32_t k = 0; k < BATCH; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+          for (uint32_t k = 0; k < B; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));  // (and every lane has read)
 #pragma unroll
-        for (uint32_t k = 0; k < BATCH; ++k) {
-          const T *e = reinterpret_cast<const T *>(raw[k]);
-          const uint32_t r = r0 + 4 * X * k, ex = __float_as_uint(top[k]) >> 23;
+        for (uint32_t k = 0; k < B; ++k) {
+          const uint32_t ex = __float_as_uint(top[k]) >> 23;
           const bool fits = ex > 0 && ex < 254;
-          const float down = (r < n_rows ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : 1.f);
-          if (lane == 0) mult_s[r] = fmaxf((fits ? __uint_as_float(ex << 23) : 1.f) * pp.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
+          const float down = (r + k < n_rows ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : 1.f);
+          if (lane == 0) mult_s[r + k] = fmaxf((fits ? __uint_as_float(ex << 23) : 1.f) * pp.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
 #pragma unroll
           for (uint32_t i = 0; i < E; i += 2) {
-            const float f0 = to_f(e[i]) * down, f1 = to_f(e[i + 1]) * down;
+            const float f0 = v[k][i] * down, f1 = v[k][i + 1] * down;
             const uint32_t h = pp_pack(f0, f1), c = E * lane + i;
-            const uint32_t at = q_u + (r >> 7) * S::TERMS * QT + c / 64 * PP_PLANE + pp_sw(r & 127, c % 64 / 8) + c % 8 * 2;
+            const uint32_t at = q_u + (r >> 7) * S::TERMS * QT + c / 64 * PP_PLANE + pp_sw((r + k) & 127, c % 64 / 8) + c % 8 * 2;
             asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(h) : "memory");
             if constexpr (SPLIT) {
               const float2 f = __half22float2(u32_as_h2(h));
@@ -424,12 +436,13 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       if (any_bad)
         for (uint32_t u = 0; u < 8; ++u)
           if ((8 * t + u) * PG_UNIT < my_hi && table[(8 * t + u) >> page_shift] >= d.n_pages) gone |= 1u << u;
+      const int last = (int)(pos - key0), oldest = d.window && pos >= d.window ? (int)(pos - d.window + 1 - key0) : -1;  // keys of the tile that the row sees
       auto masked = [&](uint32_t j, uint32_t (&s)[32]) {
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-          const uint32_t key = key0 + 32 * j + i;
-          if (key > pos || (d.window && pos - key >= d.window) || (gone >> (2 * j + i / 16) & 1)) s[i] = 0xff800000u;
-        }
+        for (int i = 0; i < 32; ++i) s[i] = (i > last - 32 * (int)j) | (i < oldest - 32 * (int)j) ? 0xff800000u : s[i];
+        if (gone)
+#pragma unroll
+          for (uint32_t i = 0; i < 32; ++i) s[i] = gone >> (2 * j + i / 16) & 1 ? 0xff800000u : s[i];
       };
       float mx = -INFINITY;
 #pragma unroll 1
