@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
     }
     const uint32_t tk = 4 * (g / 2) + (g & 1);  // the token of MMA row g; row g + 8 is the second after it
     for (uint32_t i = 0; i < mine && !dead; ++i) {
-      if (!warp_wait_one(bar + 8 * stage, phase)) {
+      if (!warp_wait(bar + 8 * stage, phase)) {
         dead = true;
         break;
       }

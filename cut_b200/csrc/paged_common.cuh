@@ -66,17 +66,9 @@ __device__ __forceinline__ uint32_t paged_seq_of(const cutb_paged_desc &d, uint3
 }
 
 // This thread's warp, as a number that the compiler knows to be the same in all of its lanes.  Where roles are told apart by threadIdx.x / 32
-// it must expect lanes that have parted: a shuffle then takes 230 cycles instead of 25, and every vote and matrix instruction as much.
+// it must expect lanes that have parted: a shuffle then takes 230 cycles instead of 25, and every vote and matrix instruction as much.  (So it must
+// behind a wait that one lane makes for the others: prompts of 8192 tokens 886 us with such waits, 700 with warp_wait.)
 __device__ __forceinline__ uint32_t warp_index() { return __shfl_sync(0xffffffffu, threadIdx.x / 32, 0); }
-// A wait of a whole warp by one of its lanes.
-__device__ __forceinline__ bool warp_wait_one(uint32_t bar, uint32_t parity) {
-  bool ok = false;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait_probe_first(bar, parity);
-  ok = __any_sync(0xffffffffu, ok);
-  __syncwarp();
-  return ok;
-}
-
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f(float v) { return v; }
 template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }

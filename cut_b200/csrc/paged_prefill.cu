@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     for (; unit < n_end; unit += PP_UNPACK) {
       // (a fresh barrier lets a wait on the phase before its first pass)
       const uint32_t i0 = unit / 8 - t_first, dw = unit % 8, sk = i0 % SK, pk = ~(i0 / SK) & 1, sv = i0 % SV, pv = ~(i0 / SV) & 1, next = unit + PP_UNPACK;
-      if (!warp_wait_one(kempty + sk * 8, pk) || __any_sync(0xffffffffu, aborted())) {
+      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(kempty + sk * 8, pk) && !aborted())) {
         if (lane == 0) give_up();
         break;
       }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       __syncwarp();
       if (lane == 0) mbar_arrive(kfull + sk * 8);
       if (next < n_end) load_keys(next);
-      if (!warp_wait_one(vempty + sv * 8, pv) || __any_sync(0xffffffffu, aborted())) {
+      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(vempty + sv * 8, pv) && !aborted())) {
         if (lane == 0) give_up();
         break;
       }
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     for (uint32_t t = t_first; t < t_end; ++t) {
       const uint32_t key0 = t * PP_KEYS;
       if (!(key0 < my_hi && key0 + PP_KEYS > my_lo)) continue;
-      if (!warp_wait_one(sfull + x * 8, ph) || __any_sync(0xffffffffu, aborted())) {
+      if (!__all_sync(0xffffffffu, mbar_wait_probe_first(sfull + x * 8, ph) && !aborted())) {
         dead = true;
         break;
       }
@@ -438,6 +438,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
           if ((8 * t + u) * PG_UNIT < my_hi && table[(8 * t + u) >> page_shift] >= d.n_pages) gone |= 1u << u;
       const int last = (int)(pos - key0), oldest = d.window && pos >= d.window ? (int)(pos - d.window + 1 - key0) : -1;  // keys of the tile that the row sees
       auto masked = [&](uint32_t j, uint32_t (&s)[32]) {
+        asm volatile("" ::: "memory");  // (a branch: as selects it would be carried out for every tile)
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[i] = (i > last - 32 * (int)j) | (i < oldest - 32 * (int)j) ? 0xff800000u : s[i];
         if (gone)
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       // The weighted values follow.  Those of fp32 rows leave the tensor cores after every tile and are added here: a sum that goes on
       // there loses half a unit of its last place at every product of 16 keys.
       if (done && (rises || SPLIT)) {
-        if (!warp_wait_one(odone + x * 8, (done - 1) & 1u)) {
+        if (!warp_wait(odone + x * 8, (done - 1) & 1u)) {
           dead = true;
           break;
         }
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       }
       ++done;
     }
-    if (!dead && done && !warp_wait_one(odone + x * 8, (done - 1) & 1u)) dead = true;
+    if (!dead && done && !warp_wait(odone + x * 8, (done - 1) & 1u)) dead = true;
     if (dead) {
       if (lane == 0) give_up();
     } else if (done) {
