@@ -1,19 +1,32 @@
 // The next token of each row of logits, by a given random number.
+//
+// A cluster of 1 to 8 blocks works on a row.  A block keeps its part as fp32 in shared memory, or where that would leave one block on
+// an SM reads it again from L2.  Weights are
+// integers of 2^-42 of the largest, so that sums do not depend on the order of additions and blocks (fp32 weights would
+// move a choice among a hundred thousand even ones once in a few hundred draws).
+// The cut-offs are places in the falling order: the key (a logit's bits as an ordered integer) where a count or a sum of weights has
+// gone by is found 11 bits at a time.  Each step is a histogram of 2048 places in shared memory, 32-bit additions only (a weight as three
+// times 16 bits, at most 2^16 elements to a block); every block then adds up the cluster's histograms for itself, so a step is one cluster
+// barrier.  Equal logits are cut off by their index.  The draw adds up the kept weights in the order of the indices.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
 #include "kernels.h"
 #include "paged_common.cuh"
 
 namespace cutb {
 namespace {
 
-constexpr uint32_t SM_THREADS = 1024, SM_WARPS = 32;
-constexpr double SM_ONE = 4398046511104.0;  // 2^42: weights are added as integers of 2^-42, up to 2^20 of them
+namespace cg = cooperative_groups;
+
+constexpr uint32_t SM_THREADS = 512, SM_WARPS = 16, SM_BINS = 2048;
+constexpr uint32_t SM_VOCAB = 1u << 19;        // an eighth of it is 2^16 elements to a block: their 16-bit pieces add up in 32 bits
+constexpr double SM_ONE = 4398046511104.0;  // 2^42
 typedef unsigned long long u64;
 
 // A logit as it counts: a NaN is minus infinity, minus zero is zero.
-template <typename T> __device__ __forceinline__ float sm_logit(const T *x, uint32_t i) {
-  const float v = to_f(x[i]) + 0.f;
-  return v != v ? -INFINITY : v;
-}
+__device__ __forceinline__ float sm_logit(float v) { return v != v ? -INFINITY : v + 0.f; }
 // larger logits have larger keys
 __device__ __forceinline__ uint32_t sm_key(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -21,29 +34,31 @@ __device__ __forceinline__ uint32_t sm_key(float v) {
 }
 __device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-struct SmRow {
-  float top;
-  double rate;  // 1 / temperature
-  double least;
-  __device__ __forceinline__ double weight(float v) const {
-    if (v == top) return 1.0;  // (an infinite one too)
-    return exp(((double)v - (double)top) * rate);
-  }
-  __device__ __forceinline__ u64 mass(float v) const { return (u64)__double2ll_rn(weight(v) * SM_ONE); }
+struct SmShared {
+  double powers[256];  // 2^43 2^(i / 256)
+  u64 sums[SM_WARPS], part[4], before_s;
+  uint32_t words[SM_WARPS], max_s, found_s, bin_s, tally[4];
+  u64 left_s, bin_sum;
 };
 
-// Sum over the block, to all of its threads.
-__device__ __forceinline__ u64 sm_sum(u64 v, u64 *warps) {
-#pragma unroll
-  for (int o = 16; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x / 32] = v;
-  __syncthreads();
-  u64 t = warps[threadIdx.x & 31];
-#pragma unroll
-  for (int o = 16; o; o /= 2) t += __shfl_xor_sync(0xffffffffu, t, o);
-  return t;
-}
+struct SmRow {
+  float top;
+  double rate, offset;   // log2(e) / temperature, and it times the largest logit
+  const double *powers;  // 2^43 2^(i / 256)
+  // exp((v - top) / temperature) in units of 2^-42, rounded: 2^t = 2^n 2^(i / 256) (1 + c), c = exp(r ln 2) - 1 to its third power for |r| <=
+  // 1 / 512 (2^-42 is left).  Eight operations in 64 bits; with pairs of fp32 numbers it were 45 in all.
+  __device__ __forceinline__ u64 mass(float v) const {
+    if (v == top) return 1ull << 42;  // (an infinite one too)
+    const double t = fma((double)v, rate, -offset);
+    if (!(t > -44.0)) return 0;  // (and minus infinity)
+    constexpr double BIG = 6755399441055744.0 / 256.0;  // 3 * 2^51 / 256: the last place of a sum with it is 1 / 256
+    const double s = t + BIG, r = t - (s - BIG);
+    const int k = __double2loint(s);
+    const double p = powers[k & 255], c = r * fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531);
+    const u64 m = (u64)__double_as_longlong(fma(p, c, p + 4503599627370496.0)) & 0xfffffffffffffull;  // the last place of 2^52 is 1
+    return ((m >> -(k >> 8)) + 1) >> 1;
+  }
+};
 
 // What is kept so far: keys above `key`, and of those equal to it the ones up to index `last`.
 struct SmCut {
@@ -51,144 +66,296 @@ struct SmCut {
   __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= last); }
 };
 
-// The first index, counted over the places where `counts(i)` is above zero, at which the running sum passes `target`: warps take
-// consecutive parts, the one where it happens walks its part.
-template <typename F> __device__ uint32_t sm_find(uint32_t n, u64 target, u64 *warps, uint32_t *found, F counts) {
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, part = (n + SM_WARPS - 1) / SM_WARPS, a = min(n, warp * part), b = min(n, a + part);
-  u64 sum = 0;
-  for (uint32_t i = a + lane; i < b; i += 32) sum += counts(i);
+__device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
-  for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if (lane == 0) warps[warp] = sum;
-  if (threadIdx.x == 0) *found = 0xffffffffu;
-  __syncthreads();
-  u64 before = 0;
-  for (uint32_t w = 0; w < warp; ++w) before += warps[w];
-  if (before <= target && target < before + sum) {
-    for (uint32_t i0 = a; i0 < b; i0 += 32) {
-      u64 x = i0 + lane < b ? counts(i0 + lane) : 0;
+  for (int o = 16; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ u64 warp_before(u64 v) {  // sum of the lanes up to and with this one
+  const uint32_t lane = threadIdx.x & 31;
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, before + x > target);
-      if (past) {
-        if (lane == 0) *found = i0 + __ffs(past) - 1;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, x, 31);
-    }
+  for (int o = 1; o < 32; o *= 2) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= (uint32_t)o) v += y;
   }
-  __syncthreads();
-  return *found;
+  return v;
 }
 
-// One block per row.
-template <typename T> __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const __grid_constant__ cutb_sample_desc d) {
-  __shared__ u64 warps[SM_WARPS], bins[256], left_s;
-  __shared__ uint32_t found_s, digit_s;
+// RESIDENT: the block's part of the row is in shared memory; else it is read again, from L2
+template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const __grid_constant__ cutb_sample_desc d, uint32_t part) {
+  extern __shared__ __align__(16) uint8_t sm_raw[];
+  __shared__ SmShared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), r = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = warp_index();
+  float *x_s = reinterpret_cast<float *>(sm_raw);
+  uint32_t *hist = reinterpret_cast<uint32_t *>(sm_raw + (RESIDENT ? (part * 4 + 15) / 16 * 16 : 0));  // two of three times SM_BINS
+  if (tid < 256) sh.powers[tid] = exp2(43.0 + tid / 256.0);
+  if (tid == 0) sh.max_s = 0;
   pdl_enter();
-  const uint32_t r = blockIdx.x, n = d.vocab, tid = threadIdx.x;
-  const T *x = reinterpret_cast<const T *>(d.logits) + r * d.ld;
+  __syncthreads();
+  const uint32_t a = min(d.vocab, rank * part), n = min(d.vocab, a + part) - a;  // this block's part: a .. a + n - 1
+  const T *src = reinterpret_cast<const T *>(d.logits) + r * d.ld + a;
   const float temp = d.temperature ? d.temperature[r] : 1.f, p = d.top_p ? d.top_p[r] : 1.f, least = d.min_p ? d.min_p[r] : 0.f, u = d.u[r];
   const uint32_t k = d.top_k ? d.top_k[r] : 0;
   const bool bad = !(temp >= 0.f && temp < INFINITY) || p != p || least != least || !(u >= 0.f && u < 1.f);
   uint32_t best = 0;
-  for (uint32_t i = tid; i < n; i += SM_THREADS) best = max(best, sm_key(sm_logit(x, i)));
+  auto take = [&](uint32_t i, float v) {
+    v = sm_logit(v);
+    if (RESIDENT) x_s[i] = v;
+    best = max(best, sm_key(v));
+  };
+  {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t head = min(n, (uint32_t)((16 - reinterpret_cast<uintptr_t>(src) % 16) % 16 / sizeof(T))), vecs = (n - head) / V;
+    if (tid < head) take(tid, to_f(src[tid]));
+#pragma unroll 4
+    for (uint32_t i = tid; i < vecs; i += SM_THREADS) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src + head) + i);
+      const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-  for (int o = 16; o; o /= 2) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (tid == 0) found_s = 0;
-  __syncthreads();
-  if ((tid & 31) == 0) atomicMax(&found_s, best);
-  __syncthreads();
+      for (uint32_t j = 0; j < V; ++j) take(head + V * i + j, to_f(e[j]));
+    }
+    const uint32_t rest = head + V * vecs + tid;
+    if (rest < n) take(rest, to_f(src[rest]));
+  }
+  best = __reduce_max_sync(0xffffffffu, best);
+  if (lane == 0) atomicMax(&sh.max_s, best);
+  auto logit = [&](uint32_t i) { return RESIDENT ? x_s[i] : sm_logit(to_f(src[i])); };
+  cl.sync();  // (and the part is in shared memory)
+  best = 0;
+  for (uint32_t q = 0; q < C; ++q) best = max(best, *cl.map_shared_rank(&sh.max_s, q));
   SmRow row;
-  row.top = sm_value(found_s), row.rate = temp > 0.f ? 1.0 / (double)temp : 0.0, row.least = least;
-  __syncthreads();
+  const double rate = temp > 0.f ? 1.4426950408889634074 / (double)temp : 0.0;
+  row.top = sm_value(best), row.rate = rate, row.offset = rate * (double)row.top, row.powers = sh.powers;
+  const uint32_t top_key = best;
+
+  // A block's sum of `counts`, warps over consecutive chunks whose sums stay in sh.sums.
+  const uint32_t chunk = (n + SM_WARPS - 1) / SM_WARPS;
+  auto counted = [&](auto counts) {
+    const uint32_t b0 = min(n, warp * chunk), b1 = min(n, b0 + chunk);
+    u64 v = 0;
+#pragma unroll 4
+    for (uint32_t i = b0 + lane; i < b1; i += 32) v += counts(i);
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane == 0) sh.sums[warp] = v;
+    __syncthreads();
+    u64 t = 0;
+    for (uint32_t w = 0; w < SM_WARPS; ++w) t += sh.sums[w];
+    return t;
+  };
+  // Sums over the cluster: `stage` numbers the exchanges, so that none overwrites what is still read.
+  auto exchange = [&](int stage, u64 mine, u64 &before) {  // all blocks' sum; `before`: that of the blocks before this one
+    if (tid == 0) sh.part[stage] = mine;
+    cl.sync();
+    u64 total = 0;
+    before = 0;
+    for (uint32_t q = 0; q < C; ++q) {
+      const u64 v = *cl.map_shared_rank(&sh.part[stage], q);
+      if (q < rank) before += v;
+      total += v;
+    }
+    return total;
+  };
+  // The first index (of the row) at which the running sum of `counts` over this block's part passes `target`; it lies in this part, and
+  // counted(counts) came last.  The chunk where it happens is cut into one for each warp, and the warp where it happens walks its own.
+  auto locate = [&](u64 target, auto counts) {
+    uint32_t w = 0;
+    for (; w + 1 < SM_WARPS && sh.sums[w] <= target; ++w) target -= sh.sums[w];
+    const uint32_t c0 = min(n, w * chunk), c1 = min(n, c0 + chunk), each = (c1 - c0 + SM_WARPS - 1) / SM_WARPS;
+    const uint32_t b0 = min(c1, c0 + warp * each), b1 = min(c1, b0 + each);
+    u64 sum = 0;
+    for (uint32_t i = b0 + lane; i < b1; i += 32) sum += counts(i);
+    sum = warp_sum(sum);
+    __syncthreads();
+    if (lane == 0) sh.sums[warp] = sum;
+    __syncthreads();
+    u64 before = 0;
+    for (uint32_t q = 0; q < warp; ++q) before += sh.sums[q];
+    if (before <= target && target < before + sum) {
+      for (uint32_t i0 = b0; i0 < b1; i0 += 32) {
+        const u64 upto = before + warp_before(i0 + lane < b1 ? counts(i0 + lane) : 0);
+        const uint32_t past = __ballot_sync(0xffffffffu, upto > target);
+        if (past) {
+          if (lane == 0) sh.found_s = i0 + __ffs(past) - 1;
+          break;
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    __syncthreads();
+    return a + sh.found_s;
+  };
+  // the same over the cluster: every block learns the index
+  auto find = [&](int stage, u64 mine, u64 target, auto counts) {
+    u64 before;
+    (void)exchange(stage, mine, before);
+    if (before <= target && target < before + mine) {
+      const uint32_t at = locate(target - before, counts);
+      if (tid < C) cl.map_shared_rank(&sh, tid)->tally[stage] = at;
+    }
+    cl.sync();
+    return sh.tally[stage];
+  };
+
   if (bad || row.top == -INFINITY) {
-    if (tid == 0) {
+    if (rank == 0 && tid == 0) {
       if (bad) paged_report(d.status, CUTB_ERR_INVALID);
       d.tokens[r] = CUTB_NO_TOKEN;
       if (d.logprobs) d.logprobs[r] = -INFINITY;
     }
+    cl.sync();
     return;
   }
-  SmCut cut{0, n};
-  if (temp == 0.f) {
-    cut = SmCut{sm_key(row.top), sm_find(n, 0, warps, &found_s, [&](uint32_t i) { return (u64)(sm_logit(x, i) == row.top); })};
-  } else {
-    // the key whose place in the falling order is where `target` of the kept counts (or weights) has gone by, digit by digit; `left`:
-    // what of the target is left at that key
-    auto select = [&](u64 target, auto measure, u64 &left) {
-      uint32_t key = 0, mask = 0;
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) bins[tid] = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < n; i += SM_THREADS) {
-          const float v = sm_logit(x, i);
-          const uint32_t c = sm_key(v);
-          if ((c & mask) == key && cut.keeps(c, i)) atomicAdd(&bins[c >> shift & 255u], measure(v));
+  SmCut cut{0, d.vocab};
+  uint32_t buffer = 0;
+  // The key whose place in the falling order is where `target` of the kept counts (COUNT) or weights has gone by; `left`: what of the
+  // target is left at that key, `there`: what is there.
+  auto select = [&](auto count_type, u64 target, u64 &left, u64 &there) {
+    constexpr bool COUNT = decltype(count_type)::value;
+    constexpr uint32_t WORDS = COUNT ? 1 : 3;
+    uint32_t base = 0;  // of the difference to the largest key
+    for (int level = 0; level < 3; ++level) {
+      const uint32_t shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+      uint32_t *h = hist + buffer * 3 * SM_BINS;
+      buffer ^= 1;
+      for (uint32_t i = tid; i < WORDS * SM_BINS; i += SM_THREADS) h[i] = 0;
+      __syncthreads();
+      for (uint32_t i = tid; i < n; i += SM_THREADS) {
+        const float v = logit(i);
+        const uint32_t c = sm_key(v), diff = top_key - c, b = diff - base;
+        if ((level && (diff < base || b >> shift >> bits)) || !cut.keeps(c, a + i)) continue;
+        if (COUNT) {
+          atomicAdd(h + (b >> shift), 1u);
+        } else {
+          const u64 m = row.mass(v);
+          if (!m) continue;
+          atomicAdd(h + (b >> shift), (uint32_t)m & 0xffffu);
+          atomicAdd(h + SM_BINS + (b >> shift), (uint32_t)(m >> 16) & 0xffffu);
+          atomicAdd(h + 2 * SM_BINS + (b >> shift), (uint32_t)(m >> 32));
         }
-        __syncthreads();
-        if (tid == 0) {
-          int b = 255;
-          for (; b > 0 && bins[b] <= target; --b) target -= bins[b];
-          digit_s = b, left_s = target;
-        }
-        __syncthreads();
-        key |= digit_s << shift, mask |= 255u << shift, target = left_s;
       }
-      left = target;
-      return key;
-    };
-    if (k && k < n) {
-      u64 left;
-      const uint32_t key = select(k - 1, [](float) { return u64(1); }, left);
-      cut = SmCut{key, sm_find(n, left, warps, &found_s, [&](uint32_t i) { return (u64)(sm_key(sm_logit(x, i)) == key); })};
+      cl.sync();
+      u64 mine[4] = {0, 0, 0, 0};
+      for (uint32_t q = 0; q < C; ++q) {
+        const uint32_t *o = cl.map_shared_rank(h, q) + 4 * tid;
+#pragma unroll
+        for (uint32_t w = 0; w < WORDS; ++w) {
+          const uint4 e = *reinterpret_cast<const uint4 *>(o + w * SM_BINS);
+          mine[0] += (u64)e.x << 16 * w, mine[1] += (u64)e.y << 16 * w, mine[2] += (u64)e.z << 16 * w, mine[3] += (u64)e.w << 16 * w;
+        }
+      }
+      const u64 sum = mine[0] + mine[1] + mine[2] + mine[3], upto = warp_before(sum);
+      if (lane == 31) sh.sums[warp] = upto;
+      __syncthreads();
+      u64 before = upto - sum;
+      for (uint32_t w = 0; w < warp; ++w) before += sh.sums[w];
+      if (before <= target && target < before + sum) {
+        uint32_t b = 0;
+        for (; b < 3 && before + mine[b] <= target; ++b) before += mine[b];
+        sh.bin_s = 4 * tid + b, sh.left_s = target - before, sh.bin_sum = mine[b];
+      }
+      __syncthreads();
+      base += sh.bin_s << shift, target = sh.left_s, there = sh.bin_sum;
+      __syncthreads();  // (the next step writes them)
+    }
+    left = target;
+    return top_key - base;
+  };
+  if (temp == 0.f) {
+    auto f = [&](uint32_t i) { return (u64)(logit(i) == row.top); };
+    cut = SmCut{top_key, find(0, counted(f), 0, f)};
+  } else {
+    if (k && k < d.vocab) {
+      u64 left, there;
+      const uint32_t key = select(std::true_type(), k - 1, left, there);
+      cut = SmCut{key, d.vocab};
+      if (left + 1 < there) {  // some of several equal ones
+        auto f = [&](uint32_t i) { return (u64)(sm_key(logit(i)) == key); };
+        cut.last = find(0, counted(f), left, f);
+      }
     }
     if (p < 1.f) {
-      u64 total = 0;
-      for (uint32_t i = tid; i < n; i += SM_THREADS) {
-        const float v = sm_logit(x, i);
-        if (cut.keeps(sm_key(v), i)) total += row.mass(v);
-      }
-      total = sm_sum(total, warps);
+      auto f = [&](uint32_t i) {
+        const float v = logit(i);
+        return cut.keeps(sm_key(v), a + i) ? row.mass(v) : 0;
+      };
+      u64 unused;
+      const u64 total = exchange(1, counted(f), unused);
       // a token is kept while the weight before it is below the target, a number above zero
       const double want = fmax((double)p, 0.0) * (double)total;
       const u64 target = want > 1.0 ? (u64)ceil(want) - 1 : 0;
-      u64 left;
-      const uint32_t key = select(target, [&](float v) { return row.mass(v); }, left);
-      const u64 one = row.mass(sm_value(key));
-      const u64 ties = one ? left / one : 0;  // kept before the last one
-      cut = SmCut{key, sm_find(n, ties, warps, &found_s, [&](uint32_t i) {
-                    const uint32_t c = sm_key(sm_logit(x, i));
-                    return (u64)(c == key && cut.keeps(c, i));
-                  })};
+      u64 left, there;
+      const uint32_t key = select(std::false_type(), target, left, there);
+      const u64 one = row.mass(sm_value(key)), ties = one ? left / one : 0;  // kept before the last one
+      const SmCut was = cut;
+      cut = SmCut{key, key == was.key ? was.last : d.vocab};
+      if ((ties + 1) * one < there) {
+        auto g = [&](uint32_t i) {
+          const uint32_t c = sm_key(logit(i));
+          return (u64)(c == key && was.keeps(c, a + i));
+        };
+        cut.last = find(2, counted(g), ties, g);
+      }
     }
   }
-  auto kept = [&](uint32_t i) {
-    const float v = sm_logit(x, i);
-    return cut.keeps(sm_key(v), i) && (v == row.top || row.weight(v) >= row.least) ? row.mass(v) : 0;
+  const u64 fewest = least <= 0.f ? 0 : least < 1.f ? (u64)ceil((double)least * SM_ONE) : ~0ull;
+  auto kept = [&](uint32_t i) -> u64 {
+    const float v = logit(i);
+    if (!cut.keeps(sm_key(v), a + i)) return 0;
+    const u64 m = row.mass(v);
+    return v == row.top || m >= fewest ? m : 0;
   };
-  u64 total = 0;
-  for (uint32_t i = tid; i < n; i += SM_THREADS) total += kept(i);
-  total = sm_sum(total, warps);
+  const u64 mine = counted(kept);
+  u64 before;
+  const u64 total = exchange(3, mine, before);
   const u64 target = (u64)floor((double)u * (double)total);
-  const uint32_t token = sm_find(n, target, warps, &found_s, kept);
-  if (tid == 0) {
-    d.tokens[r] = token;
-    if (d.logprobs) d.logprobs[r] = temp == 0.f ? 0.f : (float)log(row.weight(sm_logit(x, token)) * (SM_ONE / (double)total));
+  if (before <= target && target < before + mine) {
+    const uint32_t token = locate(target - before, kept);
+    if (tid == 0) {
+      d.tokens[r] = token;
+      if (d.logprobs) {
+        const float v = logit(token - a);
+        d.logprobs[r] = temp == 0.f ? 0.f : (float)((v == row.top ? 0.0 : ((double)v - (double)row.top) / (double)temp) - log((double)total / SM_ONE));
+      }
+    }
   }
+  cl.sync();  // the other blocks read this one's sums
+}
+
+// Blocks of a row: more than one where the rows alone would leave SMs without work, eight at most (which is what every device can launch
+// together) and 1024 logits to each.
+uint32_t sm_cluster(uint32_t rows, uint32_t vocab, uint32_t sms) {
+  uint32_t c = 1;
+  while (c < 8 && ((uint64_t)rows * c < sms || (uint64_t)c * 65536 < vocab) && c * 1024u < vocab) c *= 2;
+  return c;
+}
+
+template <typename T, bool RESIDENT> int sm_launch(const cutb_sample_desc &d, uint32_t cluster, uint32_t part, uint32_t smem, cudaStream_t stream) {
+  CUTB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(d.rows * cluster), cfg.blockDim = dim3(SM_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 2;
+  CUTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<T, RESIDENT>, d, part));
+  return CUTB_OK;
 }
 
 }  // namespace
 
 int sample_launch(const cutb_sample_desc &d, cudaStream_t stream) {
+  DeviceInfo di;
+  if (int rc = get_device_info(&di)) return rc;
+  const uint32_t cluster = sm_cluster(d.rows, d.vocab, di.sm_count), part = ((d.vocab + cluster - 1) / cluster + 7) / 8 * 8;
+  const uint32_t hist = d.top_k || d.top_p ? 2 * 3 * SM_BINS * 4 : 0;
+  const bool resident = (uint64_t)part * 4 + hist <= 100u * 1024;  // two blocks on an SM
   return paged_with_type(d.dtype, [&](auto t) {
     using T = decltype(t);
-    CUTB_CUDA_TRY(launch_pdl(sample_kernel<T>, dim3(d.rows), dim3(SM_THREADS), 0, stream, d));
-    return (int)CUTB_OK;
+    return resident ? sm_launch<T, true>(d, cluster, part, (part * 4 + 15) / 16 * 16 + hist, stream) : sm_launch<T, false>(d, cluster, part, hist, stream);
   });
 }
 
@@ -202,8 +369,8 @@ extern "C" int cutb_sample(const cutb_sample_desc *d, void *stream) {
     return CUTB_ERR_INVALID;
   }
   if (d->rows == 0) return CUTB_OK;
-  if (d->vocab == 0 || d->vocab > (1u << 20) || (d->rows > 1 && d->ld < d->vocab) || d->rows > 0x7fffffffu) {
-    set_last_error("sample: a row has 1 .. 1048576 logits and a stride that holds them (vocab=%u ld=%llu)", d->vocab, (unsigned long long)d->ld);
+  if (d->vocab == 0 || d->vocab > SM_VOCAB || (d->rows > 1 && d->ld < d->vocab) || d->rows > (1u << 24)) {
+    set_last_error("sample: a row has 1 .. 524288 logits and a stride that holds them (vocab=%u ld=%llu)", d->vocab, (unsigned long long)d->ld);
     return CUTB_ERR_INVALID;
   }
   if (!d->logits || !d->u || !d->tokens || reinterpret_cast<uintptr_t>(d->logits) % (d->dtype == CUTB_F32 ? 4 : 2)) {

@@ -801,7 +801,7 @@ CUTB_API int cutb_pages_compact(const cutb_pages_desc *desc, void *stream);
 CUTB_API int cutb_pages_copy(const cutb_pages_desc *desc, void *stream);
 
 /*
- * The next token of each of `rows` rows of logits (dtype CUTB_F32, CUTB_F16 or CUTB_BF16, `vocab` <= 1048576 of them, rows ld elements
+ * The next token of each of `rows` rows of logits (dtype CUTB_F32, CUTB_F16 or CUTB_BF16, `vocab` <= 524288 of them, rows ld elements
  * apart) by a given random number u[r] in [0, 1) (no counterpart in the reference).  With w_i = exp((x_i - max) / temperature), tokens
  * ordered by falling logit, of equal ones the lower index first:
  *   the top_k first are kept (0: all), of those the shortest beginning that has at least top_p of their weight (1 or more: all; at

@@ -112,7 +112,7 @@ def test_sampling_that_is_refused():
     refused("cutb_sample", None, "null descriptor")
     refused("cutb_sample", s(dtype=3), "element type")
     refused("cutb_sample", s(vocab=0), "logits")
-    refused("cutb_sample", s(vocab=(1 << 20) + 1, ld=1 << 21), "logits")
+    refused("cutb_sample", s(vocab=(1 << 19) + 1, ld=1 << 21), "logits")
     refused("cutb_sample", s(ld=99), "stride")
     refused("cutb_sample", s(u=None), "null")
     refused("cutb_sample", s(tokens=None), "null")
