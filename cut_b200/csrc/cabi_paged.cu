@@ -38,6 +38,10 @@ int check_paged(const cutb_paged_desc *d, const char *what) {
     set_last_error("%s: rows and a table's tokens are counted in 31 bits", what);
     return CUTB_ERR_INVALID;
   }
+  if ((uint64_t)d->n_tokens * (2ull * d->n_kv_heads + d->n_heads) > 0x3ffffffffull) {
+    set_last_error("%s: heads of rows are counted in 34 bits", what);
+    return CUTB_ERR_INVALID;
+  }
   return CUTB_OK;
 }
 

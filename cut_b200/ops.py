@@ -519,9 +519,9 @@ _ELEMENTS = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 
 def _here(what: str, *tensors) -> None:
     """The pointers of a call belong to the current device."""
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.get_device() == torch.cuda.current_device()):
-            raise RuntimeError(f"{what}: every tensor is on the current CUDA device")
+    devices = {t.get_device() for t in tensors if t is not None}  # (-1: the host)
+    if devices and (-1 in devices or devices != {torch.cuda.current_device()}):
+        raise RuntimeError(f"{what}: every tensor is on the current CUDA device")
 
 
 def _rows(t: torch.Tensor, heads: int, head_dim: int, what: str) -> torch.Tensor:

@@ -94,6 +94,53 @@ def test_written_rows_and_their_bytes(kind, head, kv, page, rot, pairing):
     assert np.array_equal(pool[~touched], before[~touched])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("head,kv,page,rot,pairing", [(128, 16, 64, 64, 1), (128, 16, 16, 128, 0), (40, 16, 32, 6, 0), (256, 16, 16, 40, 1), (192, 16, 128, 0, 0)])
+def test_many_rows(kind, head, kv, page, rot, pairing):
+    """Enough rows for the form that writes and reads whole units, with sequences that begin and end inside of them; in every third row
+    numbers that lie halfway between two codes."""
+    from cut_b200 import ops
+
+    r = np.random.default_rng(head + rot)
+    lengths, new = [400, 37, 30, 9, 160, 1, 75, 60, 51, 90], [333, 5, 0, 9, 160, 1, 75, 22, 50, 67]
+    heads, at = 2 * kv, 3  # three rows before the first sequence
+    c = make_cache(lengths, kv, head, page, r)
+    n, t = sum(new), TYPES[kind]
+    rows = at + n + 150
+    x = r.standard_normal((rows, (heads + 2 * kv) * head))
+    x[::3] = r.integers(0, 31, x[::3].shape)
+    qkv = torch.from_numpy(x).to(t).cuda()
+    q, k, v = qkv[:, : heads * head], qkv[:, heads * head: (heads + kv) * head], qkv[:, (heads + kv) * head:]
+    cos, sin = P.tables_of(head, rot, 500)
+    q_out = torch.full((rows, heads * head), 7.0, dtype=t, device="cuda")
+    kw = dict(rot_dims=rot, pairing=pairing, cos_t=cuda(cos), sin_t=cuda(sin)) if rot else {}
+    starts = rows_of(new) + at
+    before = c.pages.clone()
+    ops.paged_kv_write(c, k, v, q=q, q_out=q_out, starts=starts, **kw)
+    ko, vo = ops.paged_kv_read(c, rows, starts=starts, dtype=torch.float32)
+    c.check()
+    x = qkv.float().cpu().numpy()
+    pos = np.concatenate([np.arange(a - b, a) for a, b in zip(lengths, new)])
+    turned = np.stack([P.turned(x[at + i, : (heads + kv) * head].reshape(-1, head), p, cos, sin, rot, pairing) for i, p in enumerate(pos)])
+    got = q_out.float().cpu().numpy()
+    assert np.array_equal(got[at: at + n], torch.from_numpy(turned[:, :heads].reshape(n, -1)).to(t).float().numpy())
+    for out, want in ((ko, turned[:, heads:]), (vo, x[at: at + n, (heads + kv) * head:].reshape(n, kv, head))):
+        out = out.cpu().numpy()
+        assert np.array_equal(out[at: at + n], P.quantised(want)[0].reshape(n, -1)) and not out[:at].any() and not out[at + n:].any()
+    assert (got[:at] == 7).all() and (got[at + n:] == 7).all()
+    # the same bytes as from rows a few at a time, and nothing else
+    whole = c.pages.clone()
+    c.pages.copy_(before)
+    cut = np.cumsum([at] + new)
+    for s, m in enumerate(new):
+        for a in range(0, m, 40):
+            part = slice(int(cut[s]) + a, int(cut[s]) + min(a + 40, m))
+            c.lengths.copy_(cuda(np.array([min(lengths[s] - m + a + 40, lengths[s]) if j == s else 0 for j in range(len(new))], dtype=np.int32)))
+            ops.paged_kv_write(c, k[part], v[part], starts=rows_of([part.stop - part.start]), slots=cuda(np.array([s], dtype=np.int32)), **kw)
+    c.check()
+    assert torch.equal(c.pages, whole)
+
+
 def test_values_that_the_cache_cannot_hold():
     from cut_b200 import _lib as L
     from cut_b200 import ops
@@ -110,6 +157,27 @@ def test_values_that_the_cache_cannot_hold():
     want, changed = P.quantised(x)
     assert changed and np.isfinite(want).all() and np.array_equal(k.cpu().numpy(), want) and torch.equal(k, v)
     c.check()
+
+
+def test_values_that_the_cache_cannot_hold_among_many_rows():
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(1)
+    n, kv = 700, 32
+    c = make_cache([n], kv, 64, 32, r)
+    x = r.standard_normal((n, kv * 64)).astype(np.float32)
+    at = r.integers(0, x.size, 400)
+    x.reshape(-1)[at] = r.choice(np.array([np.inf, -np.inf, np.nan, 1e30, -7e4, 32768.0, 1e-40], dtype=np.float32), 400)
+    x[5, :64], x[6, :32] = np.nan, np.inf
+    ops.paged_kv_write(c, cuda(x), cuda(x), starts=rows_of([n]))
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_RANGE
+    k, v = ops.paged_kv_read(c, n, starts=rows_of([n]), dtype=torch.float32)
+    c.check()
+    want = P.quantised(x.reshape(n, kv, 64))[0].reshape(n, -1)
+    assert np.isfinite(want).all() and np.array_equal(k.cpu().numpy(), want) and torch.equal(k, v)
 
 
 CASES = [  # head, query heads, kv heads, page, lengths, new rows, window
