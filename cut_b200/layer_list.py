@@ -793,6 +793,25 @@ class LayerListDecoder:
         self.check_status()
         return ids
 
+    def decode_sampled(self, seq: Sequence, logits: torch.Tensor, n: int, sampling) -> list:
+        """n tokens drawn as `sampling` (decoding.Sampling) says: the first from the last row of `logits`, what forward gave for the
+        sequence's last token, then one recorded step per further token."""
+        if not seq.greedy_ready:
+            raise RuntimeError("ask for the logits of the last token first: the continuation is drawn from them")
+        if n > 1:
+            self._check(seq, n - 1)
+
+        def feed(token):
+            seq.state[:1].copy_(token)
+            return self._one_token(seq)
+
+        picks = sampling.decode(logits, n, feed)
+        if n:
+            seq.state[:1].copy_(picks[-1:])
+        ids = picks.cpu().tolist()
+        self.check_status()
+        return ids
+
     def check_status(self) -> None:
         st = int(self.status.item())
         if st:

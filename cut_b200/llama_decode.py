@@ -24,6 +24,7 @@ import torch
 from . import _lib as L
 from . import ops, synth
 from .decoding import RecordedStep
+from .paged import PagedCache
 
 UNARY_SILU, BINARY_ADD, BINARY_MUL = 133, 0, 2  # OperatorEnum codes (operators/runtime/ComputeOpsShared.h)
 
@@ -42,6 +43,7 @@ class LlamaConfig:
     max_seq: int = 2048
     fmt: int = L.Q4_K
     kv_dtype: torch.dtype = torch.float16
+    kv_page_tokens: int = 0  # not 0: keys and values in 4 bits, in pages of 16, 32, 64, 128 or 256 tokens (paged.PagedCache), 3.2 times less than fp16
 
     @property
     def q_dim(self) -> int:
@@ -136,8 +138,10 @@ class LlamaDecoder:
         cos_t, sin_t = rope_tables(cfg)
         self.cos_t, self.sin_t = up(cos_t), up(sin_t)
         ld = (cfg.kv_dim + 3) // 4 * 4
-        self.k_cache = [torch.zeros((cfg.max_seq, ld), dtype=cfg.kv_dtype, device=self.dev) for _ in range(cfg.n_layers)]
-        self.v_cache = [torch.zeros((cfg.max_seq, ld), dtype=cfg.kv_dtype, device=self.dev) for _ in range(cfg.n_layers)]
+        self.paged = None
+        if not cfg.kv_page_tokens:
+            self.k_cache = [torch.zeros((cfg.max_seq, ld), dtype=cfg.kv_dtype, device=self.dev) for _ in range(cfg.n_layers)]
+            self.v_cache = [torch.zeros((cfg.max_seq, ld), dtype=cfg.kv_dtype, device=self.dev) for _ in range(cfg.n_layers)]
         f32 = lambda n: torch.zeros(n, dtype=torch.float32, device=self.dev)
         self.params = torch.zeros(2, dtype=torch.int32, device=self.dev)  # {pos, seqLen}
         self.token = torch.zeros(1, dtype=torch.int32, device=self.dev)
@@ -145,7 +149,15 @@ class LlamaDecoder:
         self.x = [f32(cfg.hidden), f32(cfg.hidden)]
         self.h, self.qkv, self.q_roped, self.attn = f32(cfg.hidden), f32(cfg.q_dim + 2 * cfg.kv_dim), f32(cfg.q_dim), f32(cfg.q_dim)
         self.gate, self.act, self.logits, self.next_tok = f32(cfg.ffn), f32(cfg.ffn), f32(cfg.vocab), f32(1)
-        self.attn_ws = ops.attention_workspace(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.max_seq, self.dev)
+        if cfg.kv_page_tokens:  # one sequence that holds every page, in order
+            pages = -(-cfg.max_seq // cfg.kv_page_tokens)
+            self.paged = PagedCache.allocate(pages, 1, cfg.max_seq, cfg.n_kv_heads, cfg.head_dim, cfg.n_layers, cfg.kv_page_tokens, self.dev)
+            self.paged.tables.copy_(torch.arange(pages, dtype=torch.int32).view(1, -1))
+            self.paged.refs.fill_(1)
+            self.paged.lengths, self.paged.status = self.params[1:], self.status
+            self.attn_ws = ops.paged_workspace(self.paged, cfg.n_heads, 1, torch.float32)
+        else:
+            self.attn_ws = ops.attention_workspace(cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.max_seq, self.dev)
         # fp32 activations staged at one 16-bit level per 32-k block: fp16-grade error, fp32 range
         self.act_flags = L.FLAG_ACT_16BIT if act_16bit else 0
         # overlap: which mat-vecs that directly follow a mat-vec may prefetch under their predecessor's tail (True: all).
@@ -203,13 +215,17 @@ class LlamaDecoder:
         q, k, v = self.qkv[: cfg.q_dim], self.qkv[cfg.q_dim: cfg.q_dim + cfg.kv_dim], self.qkv[cfg.q_dim + cfg.kv_dim:]
         scale = 1.0 / float(np.sqrt(np.float32(cfg.head_dim)))
         for l, lw in enumerate(self.layers):
-            kc, vc = self.k_cache[l], self.v_cache[l]
+            kc, vc = (None, None) if self.paged else (self.k_cache[l], self.v_cache[l])
             if fuse:
                 seq.append(self._matvec(self.x[0], lw["wqkv"], cfg.q_dim + 2 * cfg.kv_dim, self.qkv, norm=lw["attn_norm"], after_matvec="qkv" if l else False))
             else:
                 seq.append(rms(self.x[0], lw["attn_norm"], self.h))
                 seq.append(self._matvec(self.h, lw["wqkv"], cfg.q_dim + 2 * cfg.kv_dim, self.qkv))
-            if self.fuse_rope:
+            if self.paged:
+                seq.append(lambda l=l: self._paged_write(l, self.qkv.view(1, -1), self.q_roped.view(1, -1)))
+                seq.append(lambda l=l: ops.paged_attention(self.paged, self.q_roped.view(1, -1), cfg.n_heads, layer=l, out=self.attn.view(1, -1),
+                                                           workspace=self.attn_ws))
+            elif self.fuse_rope:
                 seq.append(lambda kc=kc, vc=vc: L.check(lib.cutb_rope_attention_decode(
                     kvd, q.data_ptr(), k.data_ptr(), v.data_ptr(), self.params.data_ptr(), self.cos_t.data_ptr(), self.sin_t.data_ptr(),
                     kc.data_ptr(), vc.data_ptr(), self.attn.data_ptr(), cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, kc.stride(0),
@@ -245,6 +261,12 @@ class LlamaDecoder:
         self._seq = seq
         # split-K mat-vecs launch a second (reduction) kernel
         self.launches_per_step = len(seq) + sum(1 for d in self._descs if d.workspace_bytes)
+
+    def _paged_write(self, l: int, qkv: torch.Tensor, q_out=None, starts=None, max_new=None) -> torch.Tensor:
+        cfg = self.cfg
+        q, k, v = qkv[:, : cfg.q_dim], qkv[:, cfg.q_dim: cfg.q_dim + cfg.kv_dim], qkv[:, cfg.q_dim + cfg.kv_dim:]
+        return ops.paged_kv_write(self.paged, k, v, q=q, q_out=q_out, starts=starts, max_new=max_new, cos_t=self.cos_t, sin_t=self.sin_t,
+                                  rot_dims=cfg.head_dim, layer=l)
 
     def weight_bytes_per_token(self) -> int:
         """Bytes of block weights one token streams (every projection once, plus the LM head)."""
@@ -292,13 +314,20 @@ class LlamaDecoder:
         q_dim, kv_dim = cfg.q_dim, cfg.kv_dim
         mm = lambda A, W, N, **kw: ops.qmatmul(A, W, cfg.fmt, N, status=self.status, flags=self.act_flags | L.FLAG_NO_OVERLAP, **kw)
         x = ops.embedding(tok, self.table, status=self.status)
+        if self.paged:
+            self.params.copy_(torch.tensor([start, start + T], dtype=torch.int32))
+            starts = torch.tensor([0, T], dtype=torch.int32).to(dev)
         for l, lw in enumerate(self.layers):
             h = ops.rmsnorm(x, lw["attn_norm"], cfg.eps)
             qkv = mm(h, lw["wqkv"], q_dim + 2 * kv_dim)
-            ops.batched_kv_write(qkv[:, q_dim: q_dim + kv_dim], qkv[:, q_dim + kv_dim:], pos, self.cos_t, self.sin_t, self.k_cache[l],
-                                 self.v_cache[l], cfg.head_dim, status=self.status)
-            att = ops.batched_attention(qkv[:, :q_dim], self.k_cache[l], self.v_cache[l], pos, self.cos_t, self.sin_t, cfg.n_heads,
-                                        cfg.n_kv_heads, cfg.head_dim, status=self.status)
+            if self.paged:
+                q = self._paged_write(l, qkv, starts=starts, max_new=T)
+                att = ops.paged_attention(self.paged, q, cfg.n_heads, starts=starts, max_new=T, layer=l)
+            else:
+                ops.batched_kv_write(qkv[:, q_dim: q_dim + kv_dim], qkv[:, q_dim + kv_dim:], pos, self.cos_t, self.sin_t, self.k_cache[l],
+                                     self.v_cache[l], cfg.head_dim, status=self.status)
+                att = ops.batched_attention(qkv[:, :q_dim], self.k_cache[l], self.v_cache[l], pos, self.cos_t, self.sin_t, cfg.n_heads,
+                                            cfg.n_kv_heads, cfg.head_dim, status=self.status)
             x = mm(att, lw["wo"], cfg.hidden, D=x, fusion_type=L.FUSION_BINARY, fusion_op=BINARY_ADD)
             h = ops.rmsnorm(x, lw["ffn_norm"], cfg.eps)
             if self.glu:
@@ -368,6 +397,27 @@ class LlamaDecoder:
             if i + 1 < n:
                 self.replay(1)
                 seq.pos += 1
+        ids = picks.cpu().tolist()
+        self.check_status()
+        return ids
+
+    def decode_sampled(self, seq: "LlamaSequence", logits: torch.Tensor, n: int, sampling) -> list:
+        """n tokens drawn as `sampling` (decoding.Sampling) says: the first from the last row of `logits`, what forward gave for the
+        sequence's last token, then one recorded step per further token."""
+        if seq.pos + n - 1 > self.cfg.max_seq:
+            raise ValueError("more tokens than the cache holds")
+
+        def feed(token):
+            self.token.copy_(token)
+            if self.graph is None:
+                self.capture()
+            self.replay(1)
+            seq.pos += 1
+            return self.logits.view(1, -1)
+
+        picks = sampling.decode(logits, n, feed)
+        if n:
+            self.token.copy_(picks[-1:])
         ids = picks.cpu().tolist()
         self.check_status()
         return ids

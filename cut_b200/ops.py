@@ -629,6 +629,13 @@ def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=
     return out
 
 
+def paged_workspace(cache, n_heads: int, n_seqs: int, dtype: torch.dtype) -> torch.Tensor:
+    """Scratch for paged_attention calls with one row of each of n_seqs sequences, for callers that keep it."""
+    d = paged_desc(cache, n_seqs, dtype)
+    d.n_heads = n_heads
+    return torch.empty(max(1, paged_workspace_bytes(d)), dtype=torch.uint8, device=cache.pages.device)
+
+
 def paged_workspace_bytes(d) -> int:
     return int(L.lib().cutb_paged_workspace_bytes(C.byref(d)))
 
