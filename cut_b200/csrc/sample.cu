@@ -26,7 +26,7 @@ constexpr double SM_ONE = 4398046511104.0;  // 2^42
 typedef unsigned long long u64;
 
 // A logit as it counts: a NaN is minus infinity, minus zero is zero.
-__device__ __forceinline__ float sm_logit(float v) { return v != v ? -INFINITY : v + 0.f; }
+__device__ __forceinline__ float sm_logit(float v) { return fmaxf(v, -INFINITY) + 0.f; }
 // larger logits have larger keys
 __device__ __forceinline__ uint32_t sm_key(float v) {
   const uint32_t b = __float_as_uint(v);
@@ -41,7 +41,7 @@ struct SmShared {
   u64 left_s, bin_sum;
 };
 
-// 2^43 2^(i / 256), summed up by the compiler
+// 2^42 2^(i / 256), summed up by the compiler
 struct SmPowers {
   double v[256];
   constexpr SmPowers() : v() {
@@ -49,7 +49,7 @@ struct SmPowers {
       const double x = i * 0.69314718055994530942 / 256;
       double term = 1, sum = 1;
       for (int k = 1; k < 24; ++k) term *= x / k, sum += term;
-      v[i] = sum * 8796093022208.0;
+      v[i] = sum * SM_ONE;
     }
   }
 };
@@ -58,19 +58,19 @@ __device__ const SmPowers sm_powers;
 struct SmRow {
   float top;
   double rate, offset;   // log2(e) / temperature, and it times the largest logit
-  const double *powers;  // 2^43 2^(i / 256)
+  const double *powers;  // 2^42 2^(i / 256)
   // exp((v - top) / temperature) in units of 2^-42, rounded: 2^t = 2^n 2^(i / 256) (1 + c), c = exp(r ln 2) - 1 to its third power for |r| <=
-  // 1 / 512 (2^-42 is left).  Eight operations in 64 bits; with pairs of fp32 numbers it were 45 in all (256 x 128256 logits, bf16: 144 us, so 129).
+  // 1 / 512 (2^-42 is left).  Ten operations in 64 bits (with pairs of fp32 numbers it were 45 in all), the ends selected without
+  // branches: 256 rows of 128256 bf16 logits without cut-offs take 68 us, where reading them takes 10.
   __device__ __forceinline__ u64 mass(float v) const {
-    if (v == top) return 1ull << 42;  // (an infinite one too)
     const double t = fma((double)v, rate, -offset);
-    if (!(t > -44.0)) return 0;  // (and minus infinity)
     constexpr double BIG = 6755399441055744.0 / 256.0;  // 3 * 2^51 / 256: the last place of a sum with it is 1 / 256
     const double s = t + BIG, r = t - (s - BIG);
     const int k = __double2loint(s);
-    const double p = powers[k & 255], c = r * fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531);
-    const u64 m = (u64)__double_as_longlong(fma(p, c, p + 4503599627370496.0)) & 0xfffffffffffffull;  // the last place of 2^52 is 1
-    return ((m >> -(k >> 8)) + 1) >> 1;
+    const double at = powers[k & 255], p = __hiloint2double(__double2hiint(at) + ((k >> 8) << 20), __double2loint(at));  // (2^n: n >= -44)
+    const double m = fma(p, r * fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531), p) + 4503599627370496.0;
+    const u64 units = (u64)__double_as_longlong(m) & 0xfffffffffffffull;  // the last place of 2^52 is 1
+    return v == top ? 1ull << 42 : t > -44.0 ? units : 0;  // (infinite logits too, and what is not a number: 0)
   }
 };
 
@@ -128,11 +128,10 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
   const float temp = d.temperature ? d.temperature[r] : 1.f, p = d.top_p ? d.top_p[r] : 1.f, least = d.min_p ? d.min_p[r] : 0.f, u = d.u[r];
   const uint32_t k = d.top_k ? d.top_k[r] : 0;
   const bool bad = !(temp >= 0.f && temp < INFINITY) || p != p || least != least || !(u >= 0.f && u < 1.f);
-  uint32_t best = 0;
+  float highest = -INFINITY;  // (fmaxf passes over what is not a number)
   auto take = [&](uint32_t i, float v) {
-    v = sm_logit(v);
-    if (RESIDENT) x_s[i] = v;
-    best = max(best, sm_key(v));
+    if (RESIDENT) x_s[i] = sm_logit(v);
+    highest = fmaxf(highest, v);
   };
   {
     constexpr uint32_t V = 16 / sizeof(T);  // elements of a load
@@ -148,7 +147,7 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
     const uint32_t rest = head + V * vecs + tid;
     if (rest < n) take(rest, to_f(src[rest]));
   }
-  best = __reduce_max_sync(0xffffffffu, best);
+  uint32_t best = __reduce_max_sync(0xffffffffu, sm_key(sm_logit(highest)));
   if (lane == 0) atomicMax(&sh.max_s, best);
   auto logit = [&](uint32_t i) { return RESIDENT ? x_s[i] : sm_logit(to_f(src[i])); };
   // f(i, logit i) for first <= i < end (first a multiple of 8) by threads me, me + step, ..
@@ -161,13 +160,14 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
     } else {
 #pragma unroll 2
       for (uint32_t i = first + V * me; i < end; i += V * step) {
-        T e[V];
-        if (i + V <= end) *reinterpret_cast<uint4 *>(e) = __ldg(reinterpret_cast<const uint4 *>(src + i));
-        else
-          for (uint32_t j = 0; j < V; ++j) e[j] = i + j < end ? src[i + j] : from_f<T>(0.f);
+        if (i + V <= end) {
+          const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src + i));
+          const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-        for (uint32_t j = 0; j < V; ++j)
-          if (i + j < end) f(i + j, sm_logit(to_f(e[j])));
+          for (uint32_t j = 0; j < V; ++j) f(i + j, sm_logit(to_f(e[j])));
+        } else {
+          for (uint32_t j = i; j < end; ++j) f(j, logit(j));
+        }
       }
     }
   };
@@ -439,21 +439,27 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
       }
     }
   }
-  auto kept = [&](uint32_t i, float v) -> u64 {
-    if (!cut.keeps(sm_key(v), a + i)) return 0;
-    const u64 m = row.mass(v);
-    return v == row.top || m >= fewest ? m : 0;
-  };
-  const u64 mine = counted(kept);
-  u64 before;
-  const u64 total = exchange(3, mine, before);
-  const u64 target = sm_share(u, total, rest);
-  if (before <= target && target < before + mine) {
-    const uint32_t token = locate(target - before, kept);
-    if (tid == 0) {
-      d.tokens[r] = token;
-      if (d.logprobs) d.logprobs[r] = temp == 0.f ? 0.f : log_share(logit(token - a), total);
+  auto draw = [&](auto kept) {
+    const u64 mine = counted(kept);
+    u64 before;
+    const u64 total = exchange(3, mine, before);
+    const u64 target = sm_share(u, total, rest);
+    if (before <= target && target < before + mine) {
+      const uint32_t token = locate(target - before, kept);
+      if (tid == 0) {
+        d.tokens[r] = token;
+        if (d.logprobs) d.logprobs[r] = temp == 0.f ? 0.f : log_share(logit(token - a), total);
+      }
     }
+  };
+  if (cut.key == 0 && fewest == 0) {
+    draw([&](uint32_t, float v) -> u64 { return row.mass(v); });
+  } else {
+    draw([&](uint32_t i, float v) -> u64 {
+      if (!cut.keeps(sm_key(v), a + i)) return 0;
+      const u64 m = row.mass(v);
+      return v == row.top || m >= fewest ? m : 0;
+    });
   }
   cl.sync();  // the other blocks read this one's sums
 }
