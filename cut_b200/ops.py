@@ -525,7 +525,7 @@ def _here(what: str, *tensors) -> None:
 
 
 def _rows(t: torch.Tensor, heads: int, head_dim: int, what: str) -> torch.Tensor:
-    if t.dtype not in _ELEMENTS or t.dim() != 2 or t.shape[1] != heads * head_dim or (t.numel() and t.stride(1) != 1):
+    if t.dtype not in _ELEMENTS or t.dim() != 2 or t.shape[1] != heads * head_dim or not (t.is_contiguous() or t.stride(1) == 1):
         raise RuntimeError(f"{what}: rows of {heads} x {head_dim} elements in float32, float16 or bfloat16, with unit stride")
     return t
 
@@ -533,7 +533,7 @@ def _rows(t: torch.Tensor, heads: int, head_dim: int, what: str) -> torch.Tensor
 def _int_vector(t: torch.Tensor | None, n: int | None, what: str):
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1) or (n is not None and t.numel() != n):
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise RuntimeError(f"{what}: an int32 vector on the device" + (f" of {n} entries" if n is not None else ""))
     return t.data_ptr()
 
@@ -579,7 +579,7 @@ def paged_kv_write(cache, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor |
         heads = q.shape[1] // hd
         _rows(q, heads, hd, "paged_kv_write: q")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif q_out.dtype != q.dtype or q_out.shape != q.shape:
             raise RuntimeError("paged_kv_write: q_out is like q")
         _rows(q_out, heads, hd, "paged_kv_write: q_out")
@@ -596,8 +596,8 @@ def paged_kv_read(cache, n_tokens: int, *, dtype: torch.dtype = torch.float16, s
     """(keys, values) [n_tokens, n_kv_heads * head_dim] that the sequences' last rows stand for in the cache; rows that no sequence has
     are zero."""
     shape = (n_tokens, cache.n_kv_heads * cache.head_dim)
-    new = torch.empty if starts is None else torch.zeros
-    k, v = (new(shape, dtype=dtype, device=cache.pages.device) for _ in range(2))
+    new = cache.pages.new_empty if starts is None else cache.pages.new_zeros
+    k, v = new(shape, dtype=dtype), new(shape, dtype=dtype)
     d = paged_desc(cache, n_tokens, dtype, starts=starts, slots=slots, max_new=max_new, layer=layer, status=status)
     d.k_out, d.ldk_out, d.v_out, d.ldv_out = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
     L.check(L.lib().cutb_paged_kv_read(C.byref(d), _stream_ptr()))
@@ -613,7 +613,7 @@ def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=
     _rows(q, n_heads, hd, "paged_attention: q")
     _here("paged_attention", q, out, workspace)
     if out is None:
-        out = torch.empty((q.shape[0], n_heads * hd), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape:
         raise RuntimeError("paged_attention: out is like q")
     _rows(out, n_heads, hd, "paged_attention: out")
@@ -623,7 +623,7 @@ def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=
     need = paged_workspace_bytes(d)
     if need:
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = q.new_empty(need, dtype=torch.uint8)
         d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     L.check(L.lib().cutb_paged_attention(C.byref(d), _stream_ptr()))
     return out
@@ -651,10 +651,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=None, top_k=Non
     _here("sample", logits, u, temperature, top_k, top_p, min_p, tokens, status)
     rows = logits.shape[0]
     if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        tokens = logits.new_empty(rows, dtype=torch.int32)
     for t, kind in ((u, torch.float32), (temperature, torch.float32), (top_p, torch.float32), (min_p, torch.float32), (top_k, torch.int32),
                     (tokens, torch.int32)):
-        if t is not None and (t.dtype != kind or t.shape != (rows,) or (rows > 1 and t.stride(0) != 1)):
+        if t is not None and (t.dtype != kind or t.shape != (rows,) or not t.is_contiguous()):
             raise RuntimeError("sample: u, temperature, top_p, min_p are float32 and top_k and tokens int32 vectors, a value per row")
     d = L.SampleDesc()
     d.logits, d.ld, d.rows, d.vocab, d.dtype = logits.data_ptr(), logits.stride(0), rows, logits.shape[1], _ELEMENTS[logits.dtype]
@@ -663,7 +663,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=None, top_k=Non
     if not want_logprobs:
         L.check(L.lib().cutb_sample(C.byref(d), _stream_ptr()))
         return tokens
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
     d.logprobs = logprobs.data_ptr()
     L.check(L.lib().cutb_sample(C.byref(d), _stream_ptr()))
     return tokens, logprobs

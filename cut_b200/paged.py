@@ -28,7 +28,7 @@ class PagedCache:
     def __init__(self, pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, *, page_tokens: int = 64,
                  n_kv_heads: int = 1, head_dim: int = 0, status: torch.Tensor | None = None):
         for t, kind, dims in ((pages, torch.uint8, 2), (tables, torch.int32, 2), (lengths, torch.int32, 1), (refs, torch.int32, 1)):
-            if t.dtype != kind or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+            if t.dtype != kind or t.dim() != dims or not (t.is_contiguous() or t.stride(-1) == 1):
                 raise RuntimeError("PagedCache: pages are uint8 [n, bytes], tables int32 [slots, n], lengths and refs int32 vectors, all with unit strides")
         if tables.shape[0] != lengths.shape[0] or refs.shape[0] != pages.shape[0] or pages.stride(0) % 16:
             raise RuntimeError("PagedCache: a length per table row, a count per page, pages on multiples of 16 bytes")
@@ -60,7 +60,7 @@ class PagedCache:
     def _vector(self, v, n: int | None = None) -> torch.Tensor:
         if not isinstance(v, torch.Tensor):
             v = torch.tensor([int(x) for x in v], dtype=torch.int32).to(self.tables.device)
-        if v.dtype != torch.int32 or v.dim() != 1 or (v.numel() > 1 and v.stride(0) != 1) or v.device != self.tables.device or (n is not None and v.numel() != n):
+        if v.dtype != torch.int32 or v.dim() != 1 or not v.is_contiguous() or v.get_device() != self.tables.get_device() or (n is not None and v.numel() != n):
             raise RuntimeError("slots, pages and counts are int32 vectors of one length on the device, or lists")
         return v
 
@@ -78,7 +78,7 @@ class PagedCache:
         ops._here(name, self.pages, self.tables, self.lengths, self.refs, self.status)
         if workspace:
             need = int(L.lib().cutb_pages_workspace_bytes(C.byref(d)))
-            ws = torch.empty(need, dtype=torch.uint8, device=self.pages.device)
+            ws = self.pages.new_empty(need)
             d.workspace, d.workspace_bytes = ws.data_ptr(), need
         L.check(getattr(L.lib(), name)(C.byref(d), ops._stream_ptr()))
 
