@@ -30,6 +30,10 @@ int check_paged(const cutb_paged_desc *d, const char *what) {
                    (unsigned long long)layer_bytes(d->n_kv_heads, d->head_dim, d->page_tokens));
     return CUTB_ERR_INVALID;
   }
+  if (misaligned(d->tables, 4) || misaligned(d->lengths, 4) || misaligned(d->slots, 4) || misaligned(d->starts, 4) || misaligned(d->status, 4)) {
+    set_last_error("%s: tables, lengths, slots, starts and the status word are 4-byte aligned", what);
+    return CUTB_ERR_INVALID;
+  }
   if (d->n_seqs > PG_MAX_SEQS || (!d->slots && d->n_seqs > d->n_slots) || (!d->starts && d->n_tokens < d->n_seqs) || (d->n_seqs && d->n_tokens && d->max_new == 0)) {
     set_last_error("%s: at most %u sequences, a slot and a row for each, and max_new at least 1", what, PG_MAX_SEQS);
     return CUTB_ERR_INVALID;
@@ -67,6 +71,10 @@ int check_pages(const cutb_pages_desc *d, const char *what, bool slots, bool mov
     set_last_error("%s: null pointer, no pages or slots, or a page that does not hold 16, 32, 64, 128 or 256 tokens", what);
     return CUTB_ERR_INVALID;
   }
+  if (misaligned(d->tables, 4) || misaligned(d->lengths, 4) || misaligned(d->refs, 4) || misaligned(d->status, 4)) {
+    set_last_error("%s: tables, lengths, refs and the status word are 4-byte aligned", what);
+    return CUTB_ERR_INVALID;
+  }
   if (moves && (!d->pages || misaligned(d->pages, 16) || d->page_bytes == 0 || d->page_bytes % 16 || d->page_bytes > (1ull << 40))) {
     set_last_error("%s: pages must be 16-byte aligned, page_bytes a multiple of 16", what);
     return CUTB_ERR_INVALID;
@@ -75,6 +83,10 @@ int check_pages(const cutb_pages_desc *d, const char *what, bool slots, bool mov
 }
 
 int check_items(const cutb_pages_desc *d, const char *what, uint32_t most, bool pairs, bool counts) {
+  if (misaligned(d->items, 4) || misaligned(d->others, 4) || misaligned(d->counts, 4)) {
+    set_last_error("%s: entries are 4-byte aligned", what);
+    return CUTB_ERR_INVALID;
+  }
   if (d->n > most || (d->n && (!d->items || (pairs && !d->others) || (counts && !d->counts)))) {
     set_last_error("%s: null entries, or more than %u of them", what, most);
     return CUTB_ERR_INVALID;
@@ -122,7 +134,7 @@ int cutb_paged_kv_write(const cutb_paged_desc *d, void *stream) {
     set_last_error("%s: the turned queries go to rows of their own", what);
     return CUTB_ERR_INVALID;
   }
-  if (d->rot_dims % 2 || d->rot_dims > d->head_dim || (d->rot_dims && (!d->cos_table || !d->sin_table || d->max_pos == 0)) || d->rot_pairing < 0 || d->rot_pairing > 1) {
+  if (d->rot_dims % 2 || d->rot_dims > d->head_dim || (d->rot_dims && (!d->cos_table || !d->sin_table || misaligned(d->cos_table, 4) || misaligned(d->sin_table, 4) || d->max_pos == 0)) || d->rot_pairing < 0 || d->rot_pairing > 1) {
     set_last_error("%s: rot_dims must be even and at most head_dim, with tables and a pairing of 0 or 1", what);
     return CUTB_ERR_INVALID;
   }

@@ -10,6 +10,9 @@
 //
 // Bound by HBM: 2560 bytes of a 128-element unit are 4096 elements, and about 290 warp instructions.  Units are copied whole by bulk
 // copies, each warp through a ring of its own, so that a block has up to 80 KB in flight and warps meet only at the ends.
+// 64 sequences of 3000 tokens, 32 heads of 128 over 8 KV heads, in bf16: 68 us, 3.6 TB/s; of 8000 in fp32: 147 us, 4.4 TB/s; 2 of 131072 in
+// fp16: 81 us, 4.2 TB/s.  Four warps to a scheduler (their registers hold the values' sums) issue in 58 % of the cycles, most of it
+// nibbles becoming fp16; a token of 1500 takes 14 us, two launches' latencies.
 // Two units a step: what a step costs besides its products (the copy, the maximum over the lanes) is paid half as often.
 // The steps of all sequences and KV heads in a row are shared out evenly over the blocks.  Where a block's part begins or ends inside
 // a KV head's units, its maxima, sums and values go to the workspace, and a second kernel joins them in their order.
@@ -476,10 +479,12 @@ template <typename T> __global__ void __launch_bounds__(PJ_THREADS) paged_join_k
   extern __shared__ float2 weight_s[];  // of part b: {largest score, sum}, then its weight
   __shared__ float warps[2][4];
   pdl_enter();
-  const uint32_t RI = plan.rows, of = gridDim.x / d.n_seqs, s = blockIdx.x / of, kvh = blockIdx.y, row = blockIdx.x % of;
   const uint32_t dp = pg_pad(d.head_dim), rep = d.n_heads / d.n_kv_heads, tid = threadIdx.x;
+  const uint32_t RI = plan.rows, token = blockIdx.x / rep, kvh = blockIdx.y, s = paged_seq_of(d, token);
+  if (s >= d.n_seqs) return;
   const PagedSeq sq = paged_seq(d, s);
-  if (row >= sq.rows * rep) return;
+  if (token - sq.row0 >= sq.rows) return;
+  const uint32_t row = blockIdx.x - sq.row0 * rep;
   const uint32_t chunks = (sq.rows * rep + RI - 1) / RI, chunk = row / RI, r = row % RI;
   const uint64_t total = plan.prefix[d.n_seqs] * d.n_kv_heads;
   uint32_t first, n;
@@ -530,6 +535,10 @@ uint32_t pt_tiles(const cutb_paged_desc &d) {
 int pt_plan(const cutb_paged_desc &d, PtPlan *p, uint64_t *bytes) {
   DeviceInfo di;
   if (int rc = get_device_info(&di)) return rc;
+  if ((uint64_t)d.n_tokens * (d.n_heads / d.n_kv_heads) > 0x7fffffffu) {
+    set_last_error("paged_attention: rows times query heads of a KV head are counted in 31 bits");
+    return CUTB_ERR_INVALID;
+  }
   const uint32_t nt = pt_tiles(d), dp = pg_pad(d.head_dim);
   p->rows = (d.dtype == CUTB_F32 ? 4 : 8) * nt;
   p->blocks = di.sm_count * (dp * nt <= 128 ? 2 : 1);
@@ -548,8 +557,7 @@ template <typename T, int DP, int NT> int pt_launch(const cutb_paged_desc &d, co
   static_assert((sizeof(T) == 4 ? 4 : 8) * NT * (DP + 4) * 4 <= pt_ring_bytes(DP) / PT_WARPS, "a warp's part fits in its ring");
   CUTB_CUDA_TRY(cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
   CUTB_CUDA_TRY(launch_pdl(paged_attention_kernel<T, DP, NT>, dim3(p.blocks), dim3(PT_THREADS), smem, stream, d, p));
-  const uint32_t rows = (d.max_new < d.n_tokens ? d.max_new : d.n_tokens) * (d.n_heads / d.n_kv_heads);
-  CUTB_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3(d.n_seqs * rows, d.n_kv_heads), dim3(PJ_THREADS), 8 * p.blocks, stream, d, p));
+  CUTB_CUDA_TRY(launch_pdl(paged_join_kernel<T>, dim3(d.n_tokens * (d.n_heads / d.n_kv_heads), d.n_kv_heads), dim3(PJ_THREADS), 8 * p.blocks, stream, d, p));
   return CUTB_OK;
 }
 

@@ -7,11 +7,13 @@
 //                   rows, weights are relative to a reference that follows the maximum in steps of 2^7, so that the weighted values are rarely
 //                   rescaled; what the scores lack to the reference is exact.
 //   issuing warp    scores = Q K^T from shared memory, weighted values = P (tensor memory) V; fp32 rows with two terms of Q and of P
-//   unpacking warps (7; 16 warps have 128 registers a thread) take turns over units of 16 tokens: nibbles from global memory (the next tile's are on their way while this one's are
-//                   turned into fp16), written as the tensor cores read them: K with a token to a row, V with an element to a row, as
+//   unpacking warps (7; 16 warps have 128 registers a thread) take turns over units of 16 tokens: nibbles from global memory (the next
+//                   tile's are on their way while this one's are turned into fp16), written as the tensor cores read them: K with a token to a row, V with an element to a row, as
 //                   its units keep four neighbouring tokens together; 128-byte swizzle.
 // A tile of 128 keys costs 256 rows of 128 elements about 2000 cycles of tensor cores, as many of exponentials, and the unpacking 800
 // issue slots a scheduler, which run beside one another: two row tiles alternate, and the weights of 64 keys at a time are handed over.
+// 8192 tokens of 32 heads (8 KV heads) of 128 in bf16: 693 us, 793 TFLOP/s of the half that is seen; 4 x 1500 behind 1500 more: 356 us; 512
+// tokens in fp32: 25 us, of which one tile's chain of products, exponentials and products is the most.
 // Every wait is bounded; on expiry the block records CUTB_ERR_TIMEOUT, frees its tensor memory and returns (it has no copies in flight).
 #include "kernels.h"
 #include "paged_common.cuh"

@@ -518,5 +518,11 @@ extern "C" int cutb_sample(const cutb_sample_desc *d, void *stream) {
     set_last_error("sample: null pointer or misaligned logits");
     return CUTB_ERR_INVALID;
   }
+  const void *words[] = {d->temperature, d->top_k, d->top_p, d->min_p, d->u, d->tokens, d->logprobs, d->status};
+  for (const void *p : words)
+    if (reinterpret_cast<uintptr_t>(p) % 4) {
+      set_last_error("sample: settings and results are 4-byte aligned");
+      return CUTB_ERR_INVALID;
+    }
   return sample_launch(*d, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -34,6 +34,8 @@ class Sampling:
     def decode(self, logits: torch.Tensor, n: int, feed) -> torch.Tensor:
         """int32 [n] on the device: the first token from the last row of `logits`, each further one from feed(the token before, a
         tensor of one element), which runs a step."""
+        if logits is None:
+            raise RuntimeError("ask for the logits of the last token first: the continuation is drawn from them")
         dev = logits.device
         kept = [torch.full((1,), v, dtype=t, device=dev) for v, t in ((self.temperature, torch.float32), (self.top_k, torch.int32),
                                                                        (self.top_p, torch.float32), (self.min_p, torch.float32))]

@@ -151,3 +151,32 @@ def test_python_refuses_tensors_that_are_not_on_the_device_or_not_alike():
         ops.sample(torch.zeros(2, 8), torch.zeros(2))
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
         ops.sample(torch.zeros(2, 8, dtype=torch.float64), torch.zeros(2))
+
+
+def test_misaligned_words_are_refused():
+    for name in CALLS:
+        for field in ("tables", "lengths", "slots", "starts", "status"):
+            refused(name, desc(**{field: 258}), "4-byte aligned")
+    refused("cutb_paged_kv_write", desc(rot_dims=128, cos_table=258, sin_table=256, max_pos=9), "tables")
+    for name in ("reserve", "fork", "free", "compact"):
+        for field in ("tables", "lengths", "refs", "status"):
+            refused("cutb_pages_" + name, pages(**{field: 258}), "4-byte aligned")
+    refused("cutb_pages_reserve", pages(counts=257), "4-byte aligned")
+    refused("cutb_pages_copy", pages(others=258), "4-byte aligned")
+    for field in ("temperature", "top_k", "top_p", "min_p", "u", "tokens", "logprobs", "status"):
+        d = L.SampleDesc()
+        for k, v in {**dict(logits=256, ld=100, rows=2, vocab=100, dtype=L.F32, u=256, tokens=256), field: 258}.items():
+            setattr(d, k, v)
+        refused("cutb_sample", d, "4-byte aligned")
+
+
+def test_more_heads_of_rows_than_are_counted():
+    for name in CALLS:
+        refused(name, desc(n_tokens=0x7fffffff, n_kv_heads=8, n_heads=32, page_bytes=1 << 30), "34 bits")
+
+
+def test_a_continuation_without_logits_is_refused():
+    from cut_b200.decoding import Sampling
+
+    with pytest.raises(RuntimeError, match="logits of the last token"):
+        Sampling().decode(None, 1, None)
