@@ -20,7 +20,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t SM_THREADS = 512, SM_WARPS = 16, SM_BINS = 2048, SM_FEW = SM_THREADS;
+constexpr uint32_t SM_THREADS = 512, SM_WARPS = 16, SM_BINS = 2048, SM_FEW = SM_THREADS, SM_LIST = SM_THREADS;
 constexpr uint32_t SM_VOCAB = 1u << 19;        // an eighth of it is 2^16 elements to a block: their 16-bit pieces add up in 32 bits
 constexpr double SM_ONE = 4398046511104.0;  // 2^42
 typedef unsigned long long u64;
@@ -37,7 +37,7 @@ __device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float
 struct SmShared {
   double powers[256];
   u64 sums[SM_WARPS], part[4], before_s;
-  uint32_t max_s, found_s, bin_s, tally[4], range[2];
+  uint32_t max_s, found_s, bin_s, many_s, tally[4], range[2];
   u64 left_s, bin_sum;
 };
 
@@ -312,18 +312,47 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
       return bin;
     };
     uint32_t *h = clear();
-    if (tid == 0) sh.range[0] = 0xffffffffu, sh.range[1] = 0;
+    if (tid == 0) sh.range[0] = 0xffffffffu, sh.range[1] = 0, sh.many_s = 0;
     sweep(0, n, tid, SM_THREADS, [&](uint32_t i, float v) {
       const uint32_t b = place(v);
       if (b < SM_BINS - 1 && cut.keeps(sm_key(v), a + i)) add(h + b, v);
     });
     const uint32_t bin = crossing(h);
     if (bin == SM_BINS) return false;
+    // the tokens at that place: the first ones into a list of the first block's (in the histogram that is not in use), and their range
+    u64 *list = reinterpret_cast<u64 *>(hist + buffer * 3 * SM_BINS), *masses = list + SM_LIST;
+    u64 *to = cl.map_shared_rank(list, 0);
+    uint32_t *many_at = cl.map_shared_rank(&sh.many_s, 0);
     sweep(0, n, tid, SM_THREADS, [&](uint32_t i, float v) {
       const uint32_t c = sm_key(v);
-      if (place(v) == bin && cut.keeps(c, a + i)) atomicMin(&sh.range[0], top_key - c), atomicMax(&sh.range[1], top_key - c);
+      if (place(v) == bin && cut.keeps(c, a + i)) {
+        atomicMin(&sh.range[0], top_key - c), atomicMax(&sh.range[1], top_key - c);
+        const uint32_t at = atomicAdd(many_at, 1u);
+        if (at < SM_LIST) to[at] = c;
+      }
     });
     cl.sync();
+    const uint32_t many = *many_at;
+    if (many <= SM_LIST) {  // few: every block compares them all (64 x 32000 fp32 logits with top-p: 37 us, 54 with steps over the keys alone)
+      const uint32_t own = tid < many ? (uint32_t)to[tid] : 0;
+      if (tid < many) masses[tid] = COUNT ? 1 : row.mass(sm_value(own));
+      if (rank && tid < many) list[tid] = own;
+      __syncthreads();
+      if (tid < many) {
+        u64 ahead = 0, same = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < many; ++j) {
+          const uint32_t o = (uint32_t)list[j];
+          const u64 m = masses[j];
+          ahead += o > own ? m : 0, same += o == own ? m : 0;
+        }
+        if (ahead <= target && target < ahead + same) sh.bin_s = own, sh.left_s = target - ahead, sh.bin_sum = same;  // (equal ones write the same)
+      }
+      __syncthreads();
+      key = sh.bin_s, left = sh.left_s, there = sh.bin_sum;
+      cl.sync();  // (the list is read)
+      return true;
+    }
     uint32_t base = 0xffffffffu, end = 0;
     for (uint32_t q = 0; q < C; ++q) base = min(base, cl.map_shared_rank(sh.range, q)[0]), end = max(end, cl.map_shared_rank(sh.range, q)[1]);
     uint32_t shift = end - base < SM_BINS ? 0 : 21 - __clz(end - base);
