@@ -131,3 +131,35 @@ def test_strides_offsets_streams_and_recordings():
         g.replay()
         torch.cuda.synchronize()
         assert tokens.tolist() == [P.sampled(row, 1.0, 0, 1.0, 0.0, a)[0] for row, a in zip(wide.double().cpu().numpy(), u.double().cpu().numpy())]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [300, 600, 5000, 40000, 128256])
+def test_counts_of_every_size(kind, vocab):
+    """Cut-offs by count on either side of what one block finishes alone, with and without the others, equal logits among them."""
+    r = np.random.default_rng(vocab + 1)
+    k = np.array([1, 2, 3, 17, 200, 255, 256, 257, 300, 511, 512, 513, 600, 1024, 2048, 5])
+    n = len(k)
+    x = 2.5 * r.standard_normal((n, vocab))
+    x[1::3] = np.round(x[1::3])  # many equal ones
+    x = torch.from_numpy(x).to(TYPES[kind]).cuda()
+    u = r.random(n).astype(np.float32)
+    check(x, u, k=k)
+    check(x, u, t=r.choice([0.01, 0.5, 1, 2, 30], n), k=k, p=r.choice([0.3, 0.9, 0.999, 1.0], n), least=r.choice([0, 0.01, 0.2], n))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_largest_logits_side_by_side(kind):
+    """The largest logits in a few threads' parts of the row, and a row whose logits but a few have no weight."""
+    r = np.random.default_rng(5)
+    vocab = 60000
+    x = r.standard_normal((8, vocab))
+    at = np.arange(vocab)
+    x[:4, at // 8 % 512 < 8] += 20
+    x[4, 20000:23000] += 20
+    x[5:, 10:] -= 1000
+    x = torch.from_numpy(x).to(TYPES[kind]).cuda()
+    u = r.random(8).astype(np.float32)
+    for k in ([50] * 8, [3, 9, 10, 11, 250, 10, 11, 12], [300, 500, 700, 900, 1100, 256, 257, 600]):
+        check(x, u, k=k)
+        check(x, u, k=k, p=[0.9] * 8, least=[0, 0.01] * 4)
