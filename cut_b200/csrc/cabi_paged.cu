@@ -162,6 +162,10 @@ int cutb_paged_attention(const cutb_paged_desc *d, void *stream) {
   if (d->n_tokens == 0 || d->n_seqs == 0) return CUTB_OK;
   if (int rc = check_rows(d, what, d->q, d->ldq, d->n_heads)) return rc;
   if (int rc = check_rows(d, what, d->out, d->ldo, d->n_heads)) return rc;
+  if ((uint64_t)d->n_tokens * (d->n_heads / d->n_kv_heads) > 0x7fffffffu) {
+    set_last_error("%s: rows times query heads of a KV head are counted in 31 bits", what);
+    return CUTB_ERR_INVALID;
+  }
   if (!(d->scale - d->scale == 0.f)) {
     set_last_error("%s: the scale must be finite", what);
     return CUTB_ERR_INVALID;
@@ -176,6 +180,10 @@ int cutb_pages_reserve(const cutb_pages_desc *d, void *stream) {
   const char *what = "pages_reserve";
   if (int rc = check_pages(d, what, true, true)) return rc;
   if (int rc = check_items(d, what, 1024, false, true)) return rc;
+  if ((uint64_t)d->n * (d->ld_table + 1) > 0xffffffffull) {
+    set_last_error("%s: the entries' tables are counted in 32 bits together", what);
+    return CUTB_ERR_INVALID;
+  }
   if (int rc = check_workspace(what, d->workspace, d->workspace_bytes, pages_workspace(*d))) return rc;
   return d->n ? pages_reserve_launch(*d, reinterpret_cast<cudaStream_t>(stream)) : (int)CUTB_OK;
 }

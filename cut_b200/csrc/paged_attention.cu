@@ -535,10 +535,6 @@ uint32_t pt_tiles(const cutb_paged_desc &d) {
 int pt_plan(const cutb_paged_desc &d, PtPlan *p, uint64_t *bytes) {
   DeviceInfo di;
   if (int rc = get_device_info(&di)) return rc;
-  if ((uint64_t)d.n_tokens * (d.n_heads / d.n_kv_heads) > 0x7fffffffu) {
-    set_last_error("paged_attention: rows times query heads of a KV head are counted in 31 bits");
-    return CUTB_ERR_INVALID;
-  }
   const uint32_t nt = pt_tiles(d), dp = pg_pad(d.head_dim);
   p->rows = (d.dtype == CUTB_F32 ? 4 : 8) * nt;
   p->blocks = di.sm_count * (dp * nt <= 128 ? 2 : 1);

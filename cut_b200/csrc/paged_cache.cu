@@ -438,8 +438,9 @@ template <typename T, bool VEC> __device__ __forceinline__ void turn_row(const c
 }
 
 // A warp per head of a piece: a whole unit is put together in shared memory, four tokens at a time, and stored in 16-byte pieces; the warps
-// behind those turn the queries.  13426 rows of 32 + 2 * 8 heads of 128 in bf16: 95 us, 56 without queries, where reading them takes 9 (34 M
-// instructions are issued then, six of ten of them in the ALU).  A warp per head of a row, bytes stored one by one, took 400.
+// behind those turn the queries.  13426 rows of 32 + 2 * 8 heads of 128 in bf16: 92 us, 50 without queries, where reading them takes 9 (some 2000
+// instructions a unit, most of them in the ALU; four blocks to an SM: with two and more rows on their way at a time 70 us).  A warp per head
+// of a row, bytes stored one by one, took 400 with the reading.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_kv_write_units_kernel(const __grid_constant__ cutb_paged_desc d) {
   __shared__ __align__(16) uint8_t stage_s[8][PC_STAGE];
   pdl_enter();
@@ -469,7 +470,7 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_
     uint8_t *scales = stage + 8 * dp;
     for (uint32_t i0 = 0; i0 < dp; i0 += 128) {
       const uint32_t i = i0 + 8 * (lane % 16), g = i / 32;
-#pragma unroll 2
+#pragma unroll 1
       for (uint32_t t0 = 0; t0 < PG_UNIT; t0 += 4) {
         const uint32_t t[2] = {t0 + second, t0 + 2 + second};
         float x[2][8];
@@ -583,14 +584,14 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_
       const uint32_t *words = reinterpret_cast<const uint32_t *>(u.codes), t0 = pos % PG_UNIT;
       T *dst = reinterpret_cast<T *>(value ? d.v_out : d.k_out) + row * ld + (uint64_t)kvh * hd;
       if (!value) {
-  #pragma unroll 4
+#pragma unroll 4
         for (uint32_t w = t0 * (dp / 8) + lane; w < (t0 + n) * (dp / 8); w += 32) {
           const uint32_t t = w / (dp / 8), at = w % (dp / 8) * 8, j = at / 32, b = at % 32 / 8;
           const __half2 sc = *reinterpret_cast<const __half2 *>(u.scales + 4 * (t * groups + j)), dd = __low2half2(sc), mm = __high2half2(sc);
           __half2 q[4];
           pg_quants(words[pg_key_word(dp, t, j, b)], q);
           float x[8];
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 f = __half22float2(__hfma2(q[k], dd, mm));
             x[2 * k] = f.x, x[2 * k + 1] = f.y;
@@ -605,19 +606,19 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_
         const __half2 *sc = reinterpret_cast<const __half2 *>(u.scales) + 4 * (i / 2 * 4 + t4 / 4);
         const __half2 d01 = sc[0], d23 = sc[1], m01 = sc[2], m23 = sc[3];
         uint32_t word[8];
-  #pragma unroll
+#pragma unroll
         for (uint32_t r = 0; r < 8; ++r) word[r] = words[pg_value_byte(t4, i, r) / 4];
-  #pragma unroll
+#pragma unroll
         for (uint32_t high = 0; high < 2; ++high) {
           float x[4][8];
-  #pragma unroll
+#pragma unroll
           for (uint32_t r = 0; r < 8; ++r) {
             __half2 q[4];
             pg_quants(word[r], q);
             const float2 a = __half22float2(__hfma2(q[high], d01, m01)), b = __half22float2(__hfma2(q[2 + high], d23, m23));
             x[0][r] = a.x, x[1][r] = a.y, x[2][r] = b.x, x[3][r] = b.y;
           }
-  #pragma unroll
+#pragma unroll
           for (uint32_t k = 0; k < 4; ++k)
             if (t4 + k >= t0 && t4 + k < t0 + n) store8<T, VEC>(dst + (uint64_t)(t4 + k - t0) * ld, 16 * i + 8 * high, hd, x[k]);
         }

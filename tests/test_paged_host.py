@@ -175,8 +175,17 @@ def test_more_heads_of_rows_than_are_counted():
         refused(name, desc(n_tokens=0x7fffffff, n_kv_heads=8, n_heads=32, page_bytes=1 << 30), "34 bits")
 
 
+def test_more_query_rows_than_are_counted():
+    refused("cutb_paged_attention", desc(n_tokens=1 << 30, n_kv_heads=1, n_heads=4, head_dim=128, ldq=512, ldo=512), "31 bits")
+
+
 def test_a_continuation_without_logits_is_refused():
     from cut_b200.decoding import Sampling
 
     with pytest.raises(RuntimeError, match="logits of the last token"):
         Sampling().decode(None, 1, None)
+
+
+def test_tables_whose_entries_would_overflow_are_refused():
+    refused("cutb_pages_reserve", pages(n=1024, ld_table=1 << 22, page_tokens=16), "32 bits")
+    refused("cutb_pages_reserve", pages(n=100, ld_table=1 << 26, page_tokens=16), "32 bits")
