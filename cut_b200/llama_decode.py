@@ -259,8 +259,8 @@ class LlamaDecoder:
             seq.append(self._matvec(self.h, self.lm_head, cfg.vocab, self.logits))
         seq.append(lambda: L.check(lib.cutb_argreduce(1, self.logits.data_ptr(), self.next_tok.data_ptr(), cfg.vocab, ops._stream_ptr())))
         self._seq = seq
-        # split-K mat-vecs launch a second (reduction) kernel
-        self.launches_per_step = len(seq) + sum(1 for d in self._descs if d.workspace_bytes)
+        # split-K mat-vecs launch a second (reduction) kernel, and attention over pages one that joins its parts
+        self.launches_per_step = len(seq) + sum(1 for d in self._descs if d.workspace_bytes) + (cfg.n_layers if self.paged else 0)
 
     def _paged_write(self, l: int, qkv: torch.Tensor, q_out=None, starts=None, max_new=None) -> torch.Tensor:
         cfg = self.cfg

@@ -410,3 +410,75 @@ def test_recorded_calls_follow_the_lengths_and_streams_stay_apart():
             for h in (0, nh - 1):
                 y, spread, products = P.attention(x[s, h * head: (h + 1) * head], ks[s][h * kv // nh], vs[s][h * kv // nh], lengths[s] - 1, 128 ** -0.5, 0)
                 assert (np.abs(got[s, h * head: (h + 1) * head] - y) <= P.tolerance(y, spread, products, 128 ** -0.5, "f32")).all()
+
+
+def test_what_is_wrong_among_many_rows_is_left_out_and_reported():
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(8)
+    kv, head, new, page = 32, 64, 120, 16
+    c = make_cache([150] * 6, kv, head, page, r)
+    good = c.tables.clone()
+    c.tables[1, 4] = 1 << 20   # a page that does not exist: tokens 64 .. 79
+    c.tables[0, 9] = -5        # tokens 144 .. 149
+    c.lengths[2] = 1 << 30     # longer than the table
+    c.lengths[3] = new - 1     # shorter than the new rows
+    slots = cuda(np.array([0, 1, 2, 3, 77, 5], dtype=np.int32))
+    k, v, q = (torch.from_numpy(r.standard_normal((6 * new + 40, kv * head)).astype(np.float32)).cuda() for _ in range(3))
+    cos, sin = P.tables_of(head, 16, 140)  # and no positions past 139
+    starts, before = rows_of([new] * 6), c.pages.clone()
+    q_out = torch.full_like(q, 7.0)
+    ops.paged_kv_write(c, k, v, q=q, q_out=q_out, starts=starts, slots=slots, max_new=new, rot_dims=16, cos_t=cuda(cos), sin_t=cuda(sin))
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_INVALID
+    ko, vo = ops.paged_kv_read(c, 6 * new + 40, starts=starts, slots=slots, max_new=new, dtype=torch.float32)
+    with pytest.raises(L.CutbError):
+        c.check()
+    ko, vo, q_out, x, y, z = (a.cpu().numpy() for a in (ko, vo, q_out, k, v, q))
+    written, bad = np.zeros(6 * new + 40, dtype=bool), np.zeros(6 * new + 40, dtype=bool)
+    for s in range(6):
+        for i in range(new):
+            pos, row = 150 - new + i, s * new + i
+            bad[row] = s in (2, 3, 4) or (s == 1 and pos // page == 4) or (s == 0 and pos // page == 9)
+            written[row] = not bad[row] and pos < 140
+            if written[row]:
+                assert np.array_equal(ko[row], P.quantised(P.turned(x[row].reshape(kv, head), pos, cos, sin, 16, 0))[0].reshape(-1)), row
+                assert np.array_equal(q_out[row], P.turned(z[row].reshape(kv, head), pos, cos, sin, 16, 0).reshape(-1)), row
+    assert np.array_equal(vo[written], P.quantised(y[written].reshape(-1, kv, head))[0].reshape(written.sum(), -1))
+    assert (q_out[~written] == 7).all() and not ko[bad].any() and not vo[bad].any() and not ko[6 * new:].any()
+    assert np.isnan(ko[: 6 * new][~written[: 6 * new] & ~bad[: 6 * new]]).all()  # the pool as it was
+    changed = (c.pages != before).any(1).nonzero().view(-1).tolist()
+    assert set(changed) <= set(good[0, 1:9].tolist()) | set(good[1, 1:4].tolist()) | set(good[1, 5:9].tolist()) | set(good[5, 1:9].tolist())
+
+
+def test_many_rows_follow_a_recording_and_pages_past_32_bits():
+    """The forms for many rows, recorded once and replayed at other lengths; pages more than 4 GB into the pool."""
+    from cut_b200 import ops
+    from cut_b200.paged import PagedCache
+
+    r = np.random.default_rng(9)
+    kv, head, page, new = 16, 128, 64, 700
+    c = PagedCache.allocate(40000, 1, 2048, kv, head, page_tokens=page)
+    assert c.pages.numel() > 6 << 30
+    ids = (39999 - 1117 * np.arange(32)).astype(np.int32)
+    c.tables[0, :32] = cuda(ids)
+    k, v = (torch.from_numpy(r.standard_normal((new, kv * head)).astype(np.float32)).cuda() for _ in range(2))
+    starts = rows_of([new])
+    c.lengths.fill_(1500)
+    ops.paged_kv_write(c, k, v, starts=starts)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.paged_kv_write(c, k, v, starts=starts)
+        ko, vo = ops.paged_kv_read(c, new, starts=starts, dtype=torch.float32)
+    for length in (700, 2048, 711):
+        c.pages.fill_(255)
+        c.lengths.fill_(length)
+        k.copy_(torch.randn_like(k)), v.copy_(torch.randn_like(v))
+        g.replay()
+        c.check()
+        for got, want in ((ko, k), (vo, v)):
+            assert np.array_equal(got.cpu().numpy(), P.quantised(want.cpu().numpy().reshape(new, kv, head))[0].reshape(new, -1)), length
+        touched = set((c.pages != 255).any(1).nonzero().view(-1).tolist())  # (a page that begins before the first row is changed in part)
+        assert touched == set(ids[(length - new) // page: -(-length // page)].tolist())
