@@ -21,7 +21,8 @@ from . import ops
 
 
 class PagedCache:
-    """Views of one pool's tensors; `allocate` makes them.  pages: uint8 [n_pages, page_bytes], of every layer the part layer_bytes();
+    """Views of one pool's tensors; `allocate` makes them.  pages: uint8 [n_pages, page_bytes], of every layer the part layer_bytes() (a
+    view of some of the layers serves ops.paged_*, but no call that copies or moves pages: those take pages whole);
     tables: int32 [slots, most pages of a sequence], -1 behind a sequence's pages; lengths: int32 [slots]; refs: int32 [n_pages], how
     many slots hold a page."""
 
@@ -66,13 +67,18 @@ class PagedCache:
 
     def _desc(self, items=None, others=None, counts=None) -> "L.PagesDesc":
         d = L.PagesDesc()
-        d.pages, d.page_bytes, d.ld_table = self.pages.data_ptr(), self.pages.stride(0), self.tables.stride(0)
+        d.pages, d.page_bytes, d.ld_table = self.pages.data_ptr(), self.pages.shape[1], self.tables.stride(0)
         d.n_pages, d.page_tokens, d.n_slots = self.pages.shape[0], self.page_tokens, self.tables.shape[0]
         d.tables, d.lengths, d.refs = self.tables.data_ptr(), self.lengths.data_ptr(), self.refs.data_ptr()
         if items is not None:
             d.n, d.items, d.others, d.counts = items.numel(), items.data_ptr(), ops._ptr(others), ops._ptr(counts)
         d.status = ops._ptr(self.status)
         return d
+
+    def _whole(self, what: str) -> None:
+        """Pages are copied from one place of the pool to the next one's, which must not be more than this cache's."""
+        if self.pages.shape[0] > 1 and self.pages.stride(0) != self.pages.shape[1]:
+            raise RuntimeError(f"{what}: pages are moved whole, and these are parts of wider ones")
 
     def _run(self, name: str, d, workspace: bool) -> None:
         ops._here(name, self.pages, self.tables, self.lengths, self.refs, self.status)
@@ -85,6 +91,7 @@ class PagedCache:
     def reserve(self, slots, counts) -> None:
         """Sequence slots[i] grows by counts[i] tokens, first come, first served, in whole entries: with too few free pages the entries
         from the first that does not fit on keep their lengths (CUTB_ERR_PAGES).  A shared last page is copied before it is written."""
+        self._whole("reserve")
         slots = self._vector(slots)
         counts = self._vector(counts, slots.numel())
         self._run("cutb_pages_reserve", self._desc(slots, counts=counts), True)
@@ -99,10 +106,12 @@ class PagedCache:
         self._run("cutb_pages_free", self._desc(slots), False)
 
     def compact(self) -> None:
+        self._whole("compact")
         self._run("cutb_pages_compact", self._desc(), True)
 
     def copy(self, src, dst) -> None:
         """Page dst[i] becomes a copy of page src[i] (tables and refs are the caller's)."""
+        self._whole("copy")
         src = self._vector(src)
         dst = self._vector(dst, src.numel())
         self._run("cutb_pages_copy", self._desc(src, dst), False)

@@ -189,3 +189,23 @@ def test_a_continuation_without_logits_is_refused():
 def test_tables_whose_entries_would_overflow_are_refused():
     refused("cutb_pages_reserve", pages(n=1024, ld_table=1 << 22, page_tokens=16), "32 bits")
     refused("cutb_pages_reserve", pages(n=100, ld_table=1 << 26, page_tokens=16), "32 bits")
+
+
+def test_pages_that_are_parts_of_wider_ones_are_not_moved():
+    """reserve (copy on write), compact and copy take a page whole: of a view of some layers that would be the neighbours' bytes too."""
+    z = lambda *shape, t=torch.int32: torch.zeros(shape, dtype=t)  # noqa: E731
+    pool = z(4, 256, t=torch.uint8)
+    for part in (pool[:, :128], pool[:, 64:192], pool[::2], pool[:, 240:]):
+        n = part.shape[0]
+        c = PagedCache(part, z(2, 2), z(2), z(n), page_tokens=16)
+        for call in (lambda: c.reserve([0], [1]), c.compact, lambda: c.copy([0], [1])):
+            with pytest.raises(RuntimeError, match="moved whole"):
+                call()
+        for call in (lambda: c.fork([0], [1]), lambda: c.free([0])):  # (these touch tables and counts only; the tensors are on the host)
+            with pytest.raises(RuntimeError, match="current CUDA device"):
+                call()
+    for whole in (pool, pool[1:3], pool[2:3, :128]):  # (of one page nothing goes to another)
+        c = PagedCache(whole, z(2, 2), z(2), z(whole.shape[0]), page_tokens=16)
+        with pytest.raises(RuntimeError, match="current CUDA device"):
+            c.reserve([0], [1])
+        assert c._desc().page_bytes == whole.shape[1]
