@@ -546,7 +546,7 @@ def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=N
     part = cache.layer_bytes() if layer else 0
     if layer < 0 or (layer and (layer + 1) * part > cache.pages.shape[1]):
         raise RuntimeError("paged: no such layer in this cache")
-    d.pages, d.page_bytes, d.ld_table = cache.pages.data_ptr() + layer * part, cache.pages.stride(0), cache.tables.stride(0)
+    d.pages, d.page_bytes, d.ld_table = cache.pages.data_ptr() + layer * part, cache.pages.stride(0), cache.tables.shape[1]
     d.n_pages, d.page_tokens, d.n_kv_heads, d.head_dim = cache.pages.shape[0], cache.page_tokens, cache.n_kv_heads, cache.head_dim
     d.tables, d.lengths, d.n_slots = cache.tables.data_ptr(), cache.lengths.data_ptr(), cache.tables.shape[0]
     d.n_tokens, d.dtype = n_tokens, _ELEMENTS[dtype]

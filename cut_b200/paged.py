@@ -33,6 +33,8 @@ class PagedCache:
                 raise RuntimeError("PagedCache: pages are uint8 [n, bytes], tables int32 [slots, n], lengths and refs int32 vectors, all with unit strides")
         if tables.shape[0] != lengths.shape[0] or refs.shape[0] != pages.shape[0] or pages.stride(0) % 16:
             raise RuntimeError("PagedCache: a length per table row, a count per page, pages on multiples of 16 bytes")
+        if tables.shape[0] > 1 and tables.stride(0) != tables.shape[1]:  # (what bounds a sequence is the distance between two tables)
+            raise RuntimeError("PagedCache: tables lie one behind the other; these are parts of wider ones")
         self.pages, self.tables, self.lengths, self.refs = pages, tables, lengths, refs
         self.page_tokens, self.n_kv_heads, self.head_dim, self.status = page_tokens, n_kv_heads, head_dim, status
 
@@ -67,7 +69,7 @@ class PagedCache:
 
     def _desc(self, items=None, others=None, counts=None) -> "L.PagesDesc":
         d = L.PagesDesc()
-        d.pages, d.page_bytes, d.ld_table = self.pages.data_ptr(), self.pages.shape[1], self.tables.stride(0)
+        d.pages, d.page_bytes, d.ld_table = self.pages.data_ptr(), self.pages.shape[1], self.tables.shape[1]
         d.n_pages, d.page_tokens, d.n_slots = self.pages.shape[0], self.page_tokens, self.tables.shape[0]
         d.tables, d.lengths, d.refs = self.tables.data_ptr(), self.lengths.data_ptr(), self.refs.data_ptr()
         if items is not None:

@@ -209,3 +209,15 @@ def test_pages_that_are_parts_of_wider_ones_are_not_moved():
         with pytest.raises(RuntimeError, match="current CUDA device"):
             c.reserve([0], [1])
         assert c._desc().page_bytes == whole.shape[1]
+
+
+def test_tables_that_are_parts_of_wider_ones_are_refused():
+    """A sequence may grow to its table's end, and compact follows every entry: beyond a view's columns those are others' entries."""
+    z = lambda *shape, t=torch.int32: torch.zeros(shape, dtype=t)  # noqa: E731
+    wide, pool = z(4, 8), z(4, 256, t=torch.uint8)
+    for tables in (wide[:, :3], wide[:, 5:], wide[::2], torch.as_strided(wide, (4, 8), (2, 1)), z(1, 8).expand(4, 8)):
+        with pytest.raises(RuntimeError, match="parts of wider ones"):
+            PagedCache(pool, tables, z(tables.shape[0]), z(4))
+    for tables in (wide, wide[1:3], wide[3:, 5:], z(4, 1)):  # (one table ends where the view does)
+        c = PagedCache(pool, tables, z(tables.shape[0]), z(4), page_tokens=16)
+        assert c._desc().ld_table == tables.shape[1]
