@@ -543,8 +543,8 @@ def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=N
     starts[i + 1] - 1 of n_tokens (None: row i).  max_new: at most so many rows of a sequence (None: as many as there are)."""
     _here("paged", cache.pages, cache.tables, cache.lengths, starts, slots, status)
     d = L.PagedDesc()
-    part = cache.layer_bytes() if layer else 0
-    if layer < 0 or (layer and (layer + 1) * part > cache.pages.shape[1]):
+    part = cache.layer_bytes() if layer or cache.pages.stride(0) != cache.pages.shape[1] else 0  # (whole pages: the call itself looks at layer 0)
+    if layer < 0 or (layer + 1) * part > cache.pages.shape[1]:
         raise RuntimeError("paged: no such layer in this cache")
     d.pages, d.page_bytes, d.ld_table = cache.pages.data_ptr() + layer * part, cache.pages.stride(0), cache.tables.shape[1]
     d.n_pages, d.page_tokens, d.n_kv_heads, d.head_dim = cache.pages.shape[0], cache.page_tokens, cache.n_kv_heads, cache.head_dim

@@ -221,3 +221,15 @@ def test_tables_that_are_parts_of_wider_ones_are_refused():
     for tables in (wide, wide[1:3], wide[3:, 5:], z(4, 1)):  # (one table ends where the view does)
         c = PagedCache(pool, tables, z(tables.shape[0]), z(4), page_tokens=16)
         assert c._desc().ld_table == tables.shape[1]
+
+
+def test_a_layer_that_a_part_of_the_pages_does_not_hold_is_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    c = PagedCache.allocate(4, 2, 200, 2, 32, n_layers=3, page_tokens=16, device="cpu")
+    part = c.layer_bytes()
+    view = lambda a, b: PagedCache(c.pages[:, a:b], c.tables, c.lengths, c.refs, page_tokens=16, n_kv_heads=2, head_dim=32)  # noqa: E731
+    for cache, layer in ((view(0, part - 16), 0), (view(part, 2 * part), 1), (view(0, 2 * part + 16), 2), (c, 3), (c, -1)):
+        with pytest.raises(RuntimeError, match="no such layer"):
+            ops.paged_desc(cache, 2, torch.float32, layer=layer)
+    for cache, layer, at in ((view(part, 2 * part), 0, part), (view(part, 3 * part), 1, 2 * part), (c, 2, 2 * part), (c, 0, 0)):
+        assert ops.paged_desc(cache, 2, torch.float32, layer=layer).pages == c.pages.data_ptr() + at
