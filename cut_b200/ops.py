@@ -540,7 +540,7 @@ def _int_vector(t: torch.Tensor | None, n: int | None, what: str):
 
 def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=None, max_new: int | None = None, layer: int = 0, status=None):
     """cutb_paged_desc of a call over `cache` (paged.PagedCache): sequence i is slot slots[i] (None: slot i), its rows are starts[i] ..
-    starts[i + 1] - 1 of n_tokens (None: row i).  max_new: at most so many rows of a sequence (None: as many as there are)."""
+    starts[i + 1] - 1 of n_tokens (None: row i, one for each sequence).  max_new: at most so many rows of a sequence (None: as many as there are)."""
     _here("paged", cache.pages, cache.tables, cache.lengths, starts, slots, status)
     d = L.PagedDesc()
     part = cache.layer_bytes() if layer or cache.pages.stride(0) != cache.pages.shape[1] else 0  # (whole pages: the call itself looks at layer 0)
@@ -550,10 +550,13 @@ def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=N
     d.n_pages, d.page_tokens, d.n_kv_heads, d.head_dim = cache.pages.shape[0], cache.page_tokens, cache.n_kv_heads, cache.head_dim
     d.tables, d.lengths, d.n_slots = cache.tables.data_ptr(), cache.lengths.data_ptr(), cache.tables.shape[0]
     d.n_tokens, d.dtype = n_tokens, _ELEMENTS[dtype]
-    d.n_seqs = starts.numel() - 1 if starts is not None else slots.numel() if slots is not None else min(n_tokens, d.n_slots)
-    if d.n_seqs < 0 or (starts is None and n_tokens < d.n_seqs):
-        raise RuntimeError("paged: starts has an entry more than there are sequences; without it every sequence has a row")
-    d.starts, d.slots = _int_vector(starts, None, "starts"), _int_vector(slots, d.n_seqs, "slots")
+    n_seqs = starts.numel() - 1 if starts is not None else slots.numel() if slots is not None else n_tokens
+    if n_seqs < 0:
+        raise RuntimeError("paged: starts has an entry more than there are sequences")
+    if starts is None and (n_tokens != n_seqs or (slots is None and n_tokens > d.n_slots)):
+        raise RuntimeError("paged: without starts there are as many rows as named slots, without those too at most as many as the cache has")
+    d.n_seqs = n_seqs
+    d.starts, d.slots = _int_vector(starts, None, "starts"), _int_vector(slots, n_seqs, "slots")
     d.max_new = (1 if starts is None else max(1, n_tokens)) if max_new is None else max_new
     st = status if status is not None else cache.status
     d.status = st.data_ptr() if st is not None else None
@@ -631,8 +634,9 @@ def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=
 
 def paged_workspace(cache, n_heads: int, n_seqs: int, dtype: torch.dtype) -> torch.Tensor:
     """Scratch for paged_attention calls with one row of each of n_seqs sequences, for callers that keep it."""
-    d = paged_desc(cache, n_seqs, dtype)
-    d.n_heads = n_heads
+    d = paged_desc(cache, 0, dtype)
+    d.n_heads, d.n_seqs, d.n_tokens = n_heads, n_seqs, n_seqs
+    d.slots = d.lengths  # (only that slots are named counts here: a call may name one more than once)
     return torch.empty(max(1, paged_workspace_bytes(d)), dtype=torch.uint8, device=cache.pages.device)
 
 

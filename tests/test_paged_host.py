@@ -233,3 +233,29 @@ def test_a_layer_that_a_part_of_the_pages_does_not_hold_is_refused(monkeypatch):
             ops.paged_desc(cache, 2, torch.float32, layer=layer)
     for cache, layer, at in ((view(part, 2 * part), 0, part), (view(part, 3 * part), 1, 2 * part), (c, 2, 2 * part), (c, 0, 0)):
         assert ops.paged_desc(cache, 2, torch.float32, layer=layer).pages == c.pages.data_ptr() + at
+
+
+def test_rows_without_a_sequence_of_their_own_are_refused(monkeypatch):
+    """Without starts a row belongs to a sequence each: rows that no slot stands for would be dropped, or come back as they were."""
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    c = PagedCache.allocate(4, 4, 200, 2, 32, page_tokens=16, device="cpu")
+    f, i32 = lambda n, w: torch.zeros(n, w), lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    for n, slots in ((10, None), (5, None), (3, i32(0, 1)), (1, i32(0, 1)), (1, i32())):
+        for call in (lambda: ops.paged_attention(c, f(n, 128), 4, slots=slots), lambda: ops.paged_kv_read(c, n, slots=slots),
+                     lambda: ops.paged_kv_write(c, f(n, 64), f(n, 64), slots=slots)):
+            with pytest.raises(RuntimeError, match="as many rows as named slots"):
+                call()
+    with pytest.raises(RuntimeError, match="an entry more"):
+        ops.paged_desc(c, 0, torch.float32, starts=i32())
+    for n, kw in ((4, {}), (3, {}), (0, {}), (2, dict(slots=i32(3, 1))), (6, dict(slots=i32(0, 1, 2, 3, 3, 3))), (10, dict(starts=i32(0, 3)))):
+        d = ops.paged_desc(c, n, torch.float32, **kw)
+        assert (d.n_tokens, d.n_seqs) == (n, 1 if "starts" in kw else n)
+
+
+def test_scratch_of_more_sequences_than_slots(monkeypatch):
+    """A call may name a slot more than once: its scratch is that of as many sequences as it names."""
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    seen = []
+    monkeypatch.setattr(ops, "paged_workspace_bytes", lambda d: seen.append((d.n_seqs, d.n_tokens, d.n_heads, bool(d.slots))) or 512)
+    c = PagedCache.allocate(4, 4, 200, 2, 32, page_tokens=16, device="cpu")
+    assert ops.paged_workspace(c, 4, 100, torch.float32).numel() == 512 and seen == [(100, 100, 4, True)]
