@@ -482,3 +482,26 @@ def test_many_rows_follow_a_recording_and_pages_past_32_bits():
             assert np.array_equal(got.cpu().numpy(), P.quantised(want.cpu().numpy().reshape(new, kv, head))[0].reshape(new, -1)), length
         touched = set((c.pages != 255).any(1).nonzero().view(-1).tolist())  # (a page that begins before the first row is changed in part)
         assert touched == set(ids[(length - new) // page: -(-length // page)].tolist())
+
+
+def test_rows_of_slots_that_cannot_be_read_are_zero():
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(12)
+    lengths, kv, head = [20, 33, 0, 7], 2, 64
+    c = make_cache(lengths, kv, head, 16, r)
+    ks, vs = fill_cache(c, lengths, kv, head, r)
+    c.tables[3, 0] = 1 << 20
+    slots = cuda(np.array([1, 77, 2, 3, 0], dtype=np.int32))  # the second is none, the third empty, the fourth's page does not exist
+    for _ in range(3):
+        junk = torch.full((10 * kv * head,), 7.0, device="cuda")  # (what the allocator hands out next)
+        del junk
+        k, v = ops.paged_kv_read(c, 5, slots=slots, dtype=torch.float32)
+        with pytest.raises(L.CutbError) as e:
+            c.check()
+        assert e.value.status == L.ERR_INVALID
+        for got, want in ((k, ks), (v, vs)):
+            got = got.cpu().numpy()
+            assert not got[1:4].any()
+            assert np.array_equal(got[0], want[1][:, -1].reshape(-1)) and np.array_equal(got[4], want[0][:, -1].reshape(-1))

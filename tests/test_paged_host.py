@@ -259,3 +259,21 @@ def test_scratch_of_more_sequences_than_slots(monkeypatch):
     monkeypatch.setattr(ops, "paged_workspace_bytes", lambda d: seen.append((d.n_seqs, d.n_tokens, d.n_heads, bool(d.slots))) or 512)
     c = PagedCache.allocate(4, 4, 200, 2, 32, page_tokens=16, device="cpu")
     assert ops.paged_workspace(c, 4, 100, torch.float32).numel() == 512 and seen == [(100, 100, 4, True)]
+
+
+def test_rows_read_are_zero_where_nothing_is_read(monkeypatch):
+    """Slots and pages that do not exist are found on the device, and their rows left as they are: not as memory happens to be."""
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda: None)
+    monkeypatch.setattr(ops.L, "check", lambda rc: None)
+    c = PagedCache.allocate(4, 4, 200, 2, 32, page_tokens=16, device="cpu")
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda self, *shape, **kw: self.new_full(shape[0], 7, **kw))
+
+    class Skips:  # a call that reads nothing
+        cutb_paged_layer_bytes = L.lib().cutb_paged_layer_bytes
+        cutb_paged_kv_read = staticmethod(lambda d, s: 0)
+
+    monkeypatch.setattr(ops.L, "lib", lambda: Skips)
+    for kw in ({}, dict(slots=torch.tensor([9, 1, 2], dtype=torch.int32)), dict(starts=torch.tensor([0, 2], dtype=torch.int32))):
+        k, v = ops.paged_kv_read(c, 3, dtype=torch.float32, **kw)
+        assert k.shape == v.shape == (3, 64) and k.is_contiguous() and v.is_contiguous() and not k.any() and not v.any()
