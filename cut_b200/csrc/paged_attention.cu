@@ -216,9 +216,10 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-e of the largest element (of numbers too small or not finite: none)
+      // 2^-e of the largest element (of numbers too small: none).  An infinite element makes every score infinite or NaN, and so the weights NaN
+      // whatever the signs: the row enters as NaN.
       const uint32_t ex = __float_as_uint(top) >> 23;
-      const float down = plan.sign * (ex > 0 && ex < 254 ? __uint_as_float((254 - ex) << 23) : 1.f), up = ex > 0 && ex < 254 ? __uint_as_float(ex << 23) : 1.f;
+      const float down = plan.sign * (ex > 0 && ex < 254 ? __uint_as_float((254 - ex) << 23) : ex == 255 ? NAN : 1.f), up = ex > 0 && ex < 254 ? __uint_as_float(ex << 23) : 1.f;
 #pragma unroll
       for (int j = 0; j < G; ++j)
 #pragma unroll
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(PT_THREADS, DP * NT <= 128 ? 2 : 1) paged_atte
       if (whole) {
         const uint32_t rr = row_a + r;
         if (i < d.head_dim)
-          reinterpret_cast<T *>(d.out)[(uint64_t)(sq.row0 + rr / rep) * d.ldo + (uint64_t)(kvh * rep + rr % rep) * d.head_dim + i] = from_f<T>(sum > 0.f ? y / sum : 0.f);
+          reinterpret_cast<T *>(d.out)[(uint64_t)(sq.row0 + rr / rep) * d.ldo + (uint64_t)(kvh * rep + rr % rep) * d.head_dim + i] = from_f<T>(sum == 0.f ? 0.f : y / sum);
       } else {
         part[r * (DP + 2) + i] = y;
         if (i == 0) part[r * (DP + 2) + DP] = top, part[r * (DP + 2) + DP + 1] = sum;
@@ -522,7 +523,7 @@ template <typename T> __global__ void __launch_bounds__(PJ_THREADS) paged_join_k
     float y = 0.f;
 #pragma unroll 8
     for (uint32_t k = 0; k < parts; ++k) y = fmaf(weight_s[k].x, part(k)[i], y);
-    out[i] = from_f<T>(sum > 0.f ? y / sum : 0.f);
+    out[i] = from_f<T>(sum == 0.f ? 0.f : y / sum);
   }
 }
 

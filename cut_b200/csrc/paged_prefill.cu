@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         for (uint32_t k = 0; k < B; ++k) {
           const uint32_t ex = __float_as_uint(top[k]) >> 23;
           const bool fits = ex > 0 && ex < 254;
-          const float down = (r + k < n_rows ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : 1.f);
+          // (an infinite element makes all weights NaN: the row enters as NaN, as in the kernel for few rows)
+          const float down = (r + k < n_rows ? pp.sign : 0.f) * (fits ? __uint_as_float((254 - ex) << 23) : ex == 255 ? NAN : 1.f);
           if (lane == 0) mult_s[r + k] = fmaxf((fits ? __uint_as_float(ex << 23) : 1.f) * pp.scale, 1.1754944e-38f);  // (above zero: minus infinity stays itself)
 #pragma unroll
           for (uint32_t i = 0; i < E; i += 2) {
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       if (lane == 0) give_up();
     } else if (done) {
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       T *out = reinterpret_cast<T *>(d.out) + token * d.ldo + head;
 #pragma unroll 1
       for (uint32_t c = 0; c < DP; c += 32) {

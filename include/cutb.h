@@ -734,7 +734,8 @@ CUTB_API int cutb_expert_down(const cutb_expert_desc *desc, void *stream);
  *                         rot_dims.  No slot may be named twice, and q_out shares no memory with q, k and v.
  *   cutb_paged_kv_read    k_out, v_out = the values that the sequences' last rows stand for in the cache
  *   cutb_paged_attention  out = attention of the (turned) queries: a row at position p sees the keys j <= p with p - j < window
- *                         (window 0: all of them); a row that sees none gives zeros.  Query head h reads KV head h / (n_heads /
+ *                         (window 0: all of them); a row that sees none gives zeros, one of a query head that
+ *                         is not finite NaN.  Query head h reads KV head h / (n_heads /
  *                         n_kv_heads).  Softmax and sums in fp32; fp32 queries and their weights enter the tensor cores as two fp16 terms,
  *                         16-bit ones as one.  `workspace`: cutb_paged_workspace_bytes(), 256-byte aligned, of no content before or after.
  *                         Calls that overlap need workspaces of their own.

@@ -505,3 +505,41 @@ def test_rows_of_slots_that_cannot_be_read_are_zero():
             got = got.cpu().numpy()
             assert not got[1:4].any()
             assert np.array_equal(got[0], want[1][:, -1].reshape(-1)) and np.array_equal(got[4], want[0][:, -1].reshape(-1))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("head,nh,kv,lengths,new", [(128, 4, 2, [90, 40, 33], 1), (128, 4, 2, [2500], 3), (64, 8, 2, [70, 300], 1), (256, 2, 1, [50], 1),
+                                                    (128, 4, 2, [300, 90], 60), (64, 4, 4, [150], 150), (192, 4, 1, [100], 40)])
+def test_queries_that_are_not_finite_give_nan(kind, head, nh, kv, lengths, new):
+    """A NaN or an infinity among a head's queries makes its row NaN, whatever the signs of the scores, and no other row."""
+    from cut_b200 import ops
+
+    r = np.random.default_rng(head + new)
+    c = make_cache(lengths, kv, head, 16, r)
+    n, tokens = len(lengths) * new, sum(lengths)
+    k = r.standard_normal((tokens, kv, head)).astype(np.float32)
+    k[:, :, 3] = -1 - np.abs(k[:, :, 3])  # (an infinite query element there: minus infinity for all keys)
+    v = r.standard_normal((tokens, kv, head)).astype(np.float32)
+    ops.paged_kv_write(c, cuda(k.reshape(tokens, -1)), cuda(v.reshape(tokens, -1)), starts=rows_of(lengths))
+    cut = np.cumsum([0] + lengths)
+    q = torch.from_numpy(r.standard_normal((n, nh, head))).to(TYPES[kind]).cuda()
+    bad = {}
+    for i, (h, at, what) in enumerate([(0, 5, np.nan), (nh - 1, 3, np.inf), (1, 9, np.inf), (1, 9, -np.inf), (0, 3, -np.inf)]):
+        row = i * 7 % n
+        q[row, h, at] = what
+        if i == 1:
+            q[row, h, :3], q[row, h, 4:] = 0, 0
+        bad.setdefault(row, set()).add(h)
+    out = ops.paged_attention(c, q.view(n, -1), nh, starts=rows_of([new] * len(lengths)), max_new=new)
+    c.check()
+    x, got, scale = q.double().cpu().numpy(), out.double().cpu().numpy().reshape(n, nh, head), float(np.float32(head ** -0.5))
+    kq, vq = P.quantised(k)[0], P.quantised(v)[0]
+    for row in range(n):
+        s = row // new
+        for h in range(nh):
+            if h in bad.get(row, ()):
+                assert np.isnan(got[row, h]).all(), (row, h)
+            elif row < 12 or row % 11 == 0:
+                ks, vs = kq[cut[s]: cut[s + 1], h * kv // nh], vq[cut[s]: cut[s + 1], h * kv // nh]
+                y, spread, products = P.attention(x[row, h], ks, vs, lengths[s] - new + row % new, scale, 0)
+                assert (np.abs(got[row, h] - y) <= P.tolerance(y, spread, products, scale, kind)).all(), (row, h)
