@@ -445,7 +445,7 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
     }
   };
 
-  if (temp == 0.f) {
+  if (temp == 0.f || least > 1.f) {  // (no weight comes up to more than the largest: its first place is kept)
     auto f = [&](uint32_t, float v) { return (u64)(v == row.top); };
     cut = SmCut{top_key, find(0, counted(f), 0, f)};
   } else {

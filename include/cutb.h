@@ -806,7 +806,7 @@ CUTB_API int cutb_pages_copy(const cutb_pages_desc *desc, void *stream);
  * apart) by a given random number u[r] in [0, 1) (no counterpart in the reference).  With w_i = exp((x_i - max) / temperature), tokens
  * ordered by falling logit, of equal ones the lower index first:
  *   the top_k first are kept (0: all), of those the shortest beginning that has at least top_p of their weight (1 or more: all; at
- *   least one), of those the ones with w_i >= min_p (at least one); the token is the first kept i, by index, whose sum of weights up to
+ *   least one), of those the ones with w_i >= min_p (at least one, the first); the token is the first kept i, by index, whose sum of weights up to
  *   and with it is above u times the sum of all kept ones.  temperature 0: the largest logit.
  * temperature, top_k, top_p, min_p: a value per row in device memory; null: 1, 0, 1, 0.  logprobs (optional): the logarithm of the
  * token's share of the kept weight.  Weights are sums of 2^-42 of the largest, exactly added: the order of the additions is of no

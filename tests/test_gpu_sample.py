@@ -163,3 +163,21 @@ def test_largest_logits_side_by_side(kind):
     for k in ([50] * 8, [3, 9, 10, 11, 250, 10, 11, 12], [300, 500, 700, 900, 1100, 256, 257, 600]):
         check(x, u, k=k)
         check(x, u, k=k, p=[0.9] * 8, least=[0, 0.01] * 4)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab", [40, 5000, 128256])
+def test_least_weights_above_the_largest_with_ties(kind, vocab):
+    """min_p above 1 leaves the first of the largest logits, at 1 all of them, whatever the other cut-offs do."""
+    r = np.random.default_rng(vocab)
+    x = r.standard_normal((12, vocab))
+    for row in range(12):
+        x[row, r.permutation(vocab)[: (2, 7, 30)[row % 3]]] = 6.0
+    x[11] = 0.0
+    x[10, [3, 17]] = np.inf
+    x = torch.from_numpy(x).to(TYPES[kind]).cuda()
+    u, least = np.linspace(0.05, 0.999, 12).astype(np.float32), [7.0, 1.0, 1.0000001] * 4
+    check(x, u, least=least)
+    check(x, u, least=least, k=[20] * 12)
+    check(x, u, least=least, p=[0.6, 0.9, 1.0, 0.0] * 3)
+    check(x, u, least=least, k=[300, 5, 0, 1000, 1, 20] * 2, p=[0.6, 0.9, 1.0, 0.01] * 3, t=[1, 0.5, 3, 0] * 3)
