@@ -262,8 +262,8 @@ template <typename T, bool RESIDENT> __global__ void __launch_bounds__(SM_THREAD
   // Places of the falling order: 2048 of the weights' exponents over 43.5 (the last: no weight).  clear() gives a histogram of WORDS times
   // SM_BINS, the two in turn; crossing() the place in the cluster's sum of them where goal(their total) is reached, `target`: what is left of
   // that there, and what is there.
-  const float scale = (float)row.rate * ((SM_BINS - 1) / 43.5f);
-  auto place = [&](float v) { return min(SM_BINS - 1, __float2uint_rd((row.top - v) * scale)); };  // (what is not a number: 0)
+  const float scale = (float)row.rate * (2 * (SM_BINS - 1) / 43.5f), half = 0.5f * row.top;  // (half the distance: two finite logits may be infinitely far apart)
+  auto place = [&](float v) { return min(SM_BINS - 1, __float2uint_rd(fmaf(-0.5f, v, half) * scale)); };  // (what is not a number: 0)
   auto clear = [&](uint32_t words) {
     uint32_t *h = hist + buffer * 3 * SM_BINS;
     buffer ^= 1;

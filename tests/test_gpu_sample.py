@@ -181,3 +181,19 @@ def test_least_weights_above_the_largest_with_ties(kind, vocab):
     check(x, u, least=least, k=[20] * 12)
     check(x, u, least=least, p=[0.6, 0.9, 1.0, 0.0] * 3)
     check(x, u, least=least, k=[300, 5, 0, 1000, 1, 20] * 2, p=[0.6, 0.9, 1.0, 0.01] * 3, t=[1, 0.5, 3, 0] * 3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_logits_further_apart_than_the_type_holds(kind):
+    """The distance of two finite logits may be past the largest number; at a high temperature both have weight."""
+    r = np.random.default_rng(9)
+    big = 3e38
+    x = r.choice([big, -big, 0.0, 1e38, -2e38], (8, 3000))
+    x[1] = -big
+    x[1, 70], x[2, :] = big, np.linspace(-big, big, 3000)
+    x[3, ::5] = -np.inf
+    x = torch.from_numpy(x).to(TYPES[kind]).cuda()
+    u, t = np.array([0.999, 0.999, 0.3, 0.9, 0.95, 0.5, 0.99, 0.999], dtype=np.float32), [big, big, 1e38, big, 2e38, 1e38, big, 3e38]
+    for kw in (dict(), dict(p=[0.99, 0.999, 0.9, 0.97, 0.95, 0.999, 0.99, 0.97]), dict(k=[2000, 60, 700, 2900, 2500, 1300, 2999, 600]),
+               dict(k=[2000, 300, 1500, 2900, 0, 511, 2999, 0], p=[0.99] * 8, least=[0, 0.1, 0.01, 0, 0, 0.001, 0, 0.1])):
+        check(x, u, t=t, **kw)
