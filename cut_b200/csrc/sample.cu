@@ -24,6 +24,7 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t SM_THREADS = 512, SM_WARPS = 16, SM_BINS = 2048, SM_LIST = SM_THREADS;
 constexpr uint32_t SM_VOCAB = 1u << 19;        // an eighth of it is 2^16 elements to a block: their 16-bit pieces add up in 32 bits
+constexpr uint32_t SM_SHARED = 100 * 1024;    // dynamic shared memory of a block, at most: two blocks on an SM
 constexpr double SM_ONE = 4398046511104.0;  // 2^42
 typedef unsigned long long u64;
 
@@ -535,7 +536,8 @@ uint32_t sm_cluster(uint32_t rows, uint32_t vocab, uint32_t sms) {
 }
 
 template <typename T, bool RESIDENT> int sm_launch(const cutb_sample_desc &d, uint32_t cluster, uint32_t part, uint32_t smem, cudaStream_t stream) {
-  CUTB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // (one limit for all calls: another thread's may be set between this call's and its launch)
+  CUTB_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, RESIDENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SM_SHARED));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(d.rows * cluster), cfg.blockDim = dim3(SM_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -555,7 +557,7 @@ int sample_launch(const cutb_sample_desc &d, cudaStream_t stream) {
   if (int rc = get_device_info(&di)) return rc;
   const uint32_t cluster = sm_cluster(d.rows, d.vocab, di.sm_count), part = ((d.vocab + cluster - 1) / cluster + 7) / 8 * 8;
   const uint32_t hist = d.top_k || d.top_p ? 2 * 3 * SM_BINS * 4 : 0;
-  const bool resident = (uint64_t)part * 4 + hist <= 100u * 1024;  // two blocks on an SM
+  const bool resident = (uint64_t)part * 4 + hist <= SM_SHARED;
   return paged_with_type(d.dtype, [&](auto t) {
     using T = decltype(t);
     return resident ? sm_launch<T, true>(d, cluster, part, (part * 4 + 15) / 16 * 16 + hist, stream) : sm_launch<T, false>(d, cluster, part, hist, stream);

@@ -197,3 +197,35 @@ def test_logits_further_apart_than_the_type_holds(kind):
     for kw in (dict(), dict(p=[0.99, 0.999, 0.9, 0.97, 0.95, 0.999, 0.99, 0.97]), dict(k=[2000, 60, 700, 2900, 2500, 1300, 2999, 600]),
                dict(k=[2000, 300, 1500, 2900, 0, 511, 2999, 0], p=[0.99] * 8, least=[0, 0.1, 0.01, 0, 0, 0.001, 0, 0.1])):
         check(x, u, t=t, **kw)
+
+
+def test_two_threads_draw_from_rows_of_different_sizes():
+    """Calls at once from two threads, one with little shared memory to a block and one with much."""
+    import ctypes as C
+    import threading
+
+    from cut_b200 import _lib as L
+
+    r = np.random.default_rng(10)
+    ready, wrong, call = threading.Barrier(2), [], L.lib().cutb_sample
+
+    def work(vocab):
+        try:
+            x = torch.from_numpy(r.standard_normal((2, vocab)).astype(np.float32)).cuda()
+            u, tokens, stream = torch.full((2,), 0.5, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+            d = L.SampleDesc(logits=x.data_ptr(), ld=vocab, rows=2, vocab=vocab, dtype=L.F32, u=u.data_ptr(), tokens=tokens.data_ptr())
+            torch.cuda.synchronize()
+            ready.wait(60)
+            codes = [call(C.byref(d), stream.cuda_stream) for _ in range(20000)]
+            stream.synchronize()
+            assert set(codes) == {L.OK}
+            assert tokens.tolist() == [P.sampled(row, 1.0, 0, 1.0, 0.0, 0.5)[0] for row in x.double().cpu().numpy()]
+        except BaseException as e:  # noqa: BLE001 (handed to the test's thread)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(vocab,)) for vocab in (100, 8000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
