@@ -46,6 +46,18 @@ class Sampling:
             ops.sample(rows, u[i: i + 1], temperature=kept[0], top_k=kept[1], top_p=kept[2], min_p=kept[3], tokens=picks[i: i + 1])
         return picks
 
+    @staticmethod
+    def ids(picks: torch.Tensor, status: torch.Tensor) -> list:
+        """The drawn tokens on the host; waits for the device.  A step without a logit above minus infinity has no token, which is an
+        error (and what the steps behind it leave in the decoder's status word, which is cleared, follows from it)."""
+        ids = picks.cpu().tolist()
+        none = next((i for i, t in enumerate(ids) if t < 0), None)
+        if none is not None:
+            st = int(status.item())
+            status.zero_()
+            raise RuntimeError(f"nothing to draw: token {none} of {len(ids)} has no logit above minus infinity" + (f" (status {st})" if st else ""))
+        return ids
+
 
 class RecordedStep:
     """A fixed sequence of launches over fixed device buffers: run eagerly, or recorded once into a CUDA graph and replayed."""

@@ -806,9 +806,9 @@ class LayerListDecoder:
             return self._one_token(seq)
 
         picks = sampling.decode(logits, n, feed)
+        ids = sampling.ids(picks, self.status)
         if n:
             seq.state[:1].copy_(picks[-1:])
-        ids = picks.cpu().tolist()
         self.check_status()
         return ids
 

@@ -416,9 +416,9 @@ class LlamaDecoder:
             return self.logits.view(1, -1)
 
         picks = sampling.decode(logits, n, feed)
+        ids = sampling.ids(picks, self.status)
         if n:
             self.token.copy_(picks[-1:])
-        ids = picks.cpu().tolist()
         self.check_status()
         return ids
 

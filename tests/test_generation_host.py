@@ -56,3 +56,14 @@ def test_a_page_of_the_decoder_is_a_page_of_the_cache():
 
     with pytest.raises(ValueError):
         PagedCache.allocate(1, 1, 16, 1, 64, page_tokens=24, device="cpu")
+
+
+def test_a_token_that_could_not_be_drawn_is_an_error():
+    status = torch.zeros(1, dtype=torch.int32)
+    assert Sampling.ids(torch.tensor([3, 0, 7], dtype=torch.int32), status) == [3, 0, 7] and Sampling.ids(torch.empty(0, dtype=torch.int32), status) == []
+    with pytest.raises(RuntimeError, match="token 1 of 2"):
+        Sampling.ids(torch.tensor([3, -1], dtype=torch.int32), status)
+    status.fill_(1)
+    with pytest.raises(RuntimeError, match="status 1"):
+        Sampling.ids(torch.tensor([-1, -1], dtype=torch.int32), status)
+    assert int(status) == 0

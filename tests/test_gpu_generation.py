@@ -202,3 +202,24 @@ def test_drawn_tokens_of_a_model_folder(tmp_path):
                        timeout=600, cwd=ROOT)
     assert r.returncode == 0, r.stderr[-2000:]
     assert json.loads(r.stdout)["tokens"] == generate(dec, prompt, 10, sampling=how)
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_logits_without_a_choice_are_an_error(n, tmp_path):
+    """A diverged model's logits give no token: neither as the only one, nor as the next step's input; the decoder serves on."""
+    import test_gpu_layer_list as T
+    from cut_b200.decoding import Sampling, generate
+    from cut_b200.llama_decode import LlamaDecoder
+    from cut_b200.models import load_model
+
+    cfg, w = model(0, 64)
+    folder = T.save_model(tmp_path / "model", T.CONFIGS["wide"], T.random_weights(T.CONFIGS["wide"], 5))
+    for dec in (LlamaDecoder(cfg, w), load_model(folder, "float32", max_seq=64)):
+        for fill in (float("nan"), -float("inf")):
+            before = generate(dec, [5, 6, 7], 4, sampling=Sampling(seed=1))
+            seq = dec.open()
+            logits = dec.forward(seq, [5, 6, 7], [2])
+            with pytest.raises(RuntimeError, match=f"token 0 of {n}"):
+                dec.decode_sampled(seq, torch.full_like(logits, fill), n, Sampling())
+            dec.close(seq)
+            assert generate(dec, [5, 6, 7], 4, sampling=Sampling(seed=1)) == before
