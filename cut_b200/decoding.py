@@ -28,8 +28,8 @@ class Sampling:
     seed: int = 0
 
     def __post_init__(self):
-        if not 0.0 <= self.temperature < float("inf") or not 0 <= self.top_k < 1 << 31 or not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
-            raise ValueError("a temperature of 0 or more, a count top_k of 0 or more, and top_p and min_p from 0 to 1")
+        if not 0.0 <= self.temperature <= torch.finfo(torch.float32).max or not 0 <= self.top_k < 1 << 31 or not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
+            raise ValueError("a temperature of 0 or more (in 32 bits), a count top_k of 0 or more, and top_p and min_p from 0 to 1")
 
     def decode(self, logits: torch.Tensor, n: int, feed) -> torch.Tensor:
         """int32 [n] on the device: the first token from the last row of `logits`, each further one from feed(the token before, a

@@ -67,3 +67,10 @@ def test_a_token_that_could_not_be_drawn_is_an_error():
     with pytest.raises(RuntimeError, match="status 1"):
         Sampling.ids(torch.tensor([-1, -1], dtype=torch.int32), status)
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("temperature", [1e39, 3.5e38, 1 << 200])
+def test_a_temperature_that_32_bits_do_not_hold_is_refused(temperature):
+    with pytest.raises(ValueError, match="32 bits"):
+        Sampling(temperature=temperature)
+    assert Sampling(temperature=3.4e38).temperature == 3.4e38
