@@ -20,7 +20,8 @@ from . import ops
 
 @dataclass
 class Sampling:
-    """How decode_sampled draws tokens (ops.sample); the same seed gives the same tokens."""
+    """How decode_sampled draws tokens (ops.sample); the same seed gives the same tokens.  A sequence's tokens use up the seed's random
+    numbers one by one, over all of its calls: a reply drawn in pieces is the one drawn at once."""
     temperature: float = 1.0
     top_k: int = 0      # 0: all
     top_p: float = 1.0
@@ -31,15 +32,15 @@ class Sampling:
         if not 0.0 <= self.temperature <= torch.finfo(torch.float32).max or not 0 <= self.top_k < 1 << 31 or not 0.0 <= self.top_p <= 1.0 or not 0.0 <= self.min_p <= 1.0:
             raise ValueError("a temperature of 0 or more (in 32 bits), a count top_k of 0 or more, and top_p and min_p from 0 to 1")
 
-    def decode(self, logits: torch.Tensor, n: int, feed) -> torch.Tensor:
+    def decode(self, logits: torch.Tensor, n: int, feed, drawn: int = 0) -> torch.Tensor:
         """int32 [n] on the device: the first token from the last row of `logits`, each further one from feed(the token before, a
-        tensor of one element), which runs a step."""
+        tensor of one element), which runs a step.  drawn: tokens that the sequence has drawn so far."""
         if logits is None:
             raise RuntimeError("ask for the logits of the last token first: the continuation is drawn from them")
         dev = logits.device
         kept = [torch.full((1,), v, dtype=t, device=dev) for v, t in ((self.temperature, torch.float32), (self.top_k, torch.int32),
                                                                        (self.top_p, torch.float32), (self.min_p, torch.float32))]
-        u = torch.rand(n, device=dev, generator=torch.Generator(device=dev).manual_seed(self.seed))
+        u = torch.rand(drawn + n, device=dev, generator=torch.Generator(device=dev).manual_seed(self.seed))[drawn:]
         picks = torch.empty(n, dtype=torch.int32, device=dev)
         for i in range(n):
             rows = logits[-1:] if i == 0 else feed(picks[i - 1: i])

@@ -253,6 +253,7 @@ class Sequence:
 
     def __init__(self):
         self.pos = 0            # host copy of the position
+        self.drawn = 0          # tokens drawn (decode_sampled)
         self.open = False
         self.greedy_ready = False
         self.step = None        # RecordedStep of one token
@@ -396,7 +397,7 @@ class LayerListDecoder:
         s.state.copy_(torch.tensor([0, -1, 0, 0], dtype=torch.int32))  # -1: no previous token
         for t in s.gru.values():
             t.zero_()
-        s.pos, s.open, s.greedy_ready = 0, True, False
+        s.pos, s.drawn, s.open, s.greedy_ready = 0, 0, True, False
         return s
 
     def close(self, s: Sequence) -> None:
@@ -805,7 +806,8 @@ class LayerListDecoder:
             seq.state[:1].copy_(token)
             return self._one_token(seq)
 
-        picks = sampling.decode(logits, n, feed)
+        picks = sampling.decode(logits, n, feed, seq.drawn)
+        seq.drawn += n
         ids = sampling.ids(picks, self.status)
         if n:
             seq.state[:1].copy_(picks[-1:])

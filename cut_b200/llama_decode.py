@@ -105,10 +105,10 @@ def synthetic_weights(cfg: LlamaConfig, seed: int = 0, distinct_layers: bool = T
 
 
 class LlamaSequence:
-    """The decoder's only sequence place: how far it is."""
+    """The decoder's only sequence place: how far it is, and how many of its tokens were drawn."""
 
     def __init__(self):
-        self.pos, self.open = 0, True
+        self.pos, self.drawn, self.open = 0, 0, True
 
 
 class LlamaDecoder:
@@ -415,7 +415,8 @@ class LlamaDecoder:
             seq.pos += 1
             return self.logits.view(1, -1)
 
-        picks = sampling.decode(logits, n, feed)
+        picks = sampling.decode(logits, n, feed, seq.drawn)
+        seq.drawn += n
         ids = sampling.ids(picks, self.status)
         if n:
             self.token.copy_(picks[-1:])

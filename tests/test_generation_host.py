@@ -74,3 +74,20 @@ def test_a_temperature_that_32_bits_do_not_hold_is_refused(temperature):
     with pytest.raises(ValueError, match="32 bits"):
         Sampling(temperature=temperature)
     assert Sampling(temperature=3.4e38).temperature == 3.4e38
+
+
+def test_a_sequence_uses_up_its_seeds_numbers(monkeypatch):
+    """What is drawn in pieces is drawn by the numbers that follow, not by the first ones again."""
+    from cut_b200 import decoding
+
+    seen = []
+    monkeypatch.setattr(decoding.ops, "sample", lambda rows, u, *, tokens, **kw: (seen.append(float(u)), tokens.zero_()))
+    logits, feed = torch.zeros(1, 4), lambda token: torch.zeros(1, 4)
+    how = Sampling(seed=4)
+    assert how.decode(logits, 12, feed).tolist() == [0] * 12
+    at_once, at = list(seen), 0
+    seen.clear()
+    for n in (1, 1, 0, 5, 1, 4):
+        how.decode(logits, n, feed, at)
+        at += n
+    assert seen == at_once and len(set(seen)) == 12

@@ -223,3 +223,26 @@ def test_logits_without_a_choice_are_an_error(n, tmp_path):
                 dec.decode_sampled(seq, torch.full_like(logits, fill), n, Sampling())
             dec.close(seq)
             assert generate(dec, [5, 6, 7], 4, sampling=Sampling(seed=1)) == before
+
+
+def test_replies_drawn_in_pieces(tmp_path):
+    """Token by token, or a few at a time, with the logits of every piece's last token asked for: the reply that is drawn at once."""
+    import test_gpu_layer_list as T
+    from cut_b200.decoding import Sampling, generate
+    from cut_b200.llama_decode import LlamaDecoder
+    from cut_b200.models import load_model
+
+    cfg, w = model(16, 64)
+    folder = T.save_model(tmp_path / "model", T.CONFIGS["wide"], T.random_weights(T.CONFIGS["wide"], 5))
+    for dec in (LlamaDecoder(cfg, w), load_model(folder, "float32", max_seq=64)):
+        for how in (Sampling(temperature=3.0, seed=8), Sampling(temperature=2.0, top_k=50, seed=9)):
+            want = generate(dec, [5, 6, 7], 16, sampling=how)
+            for pieces in ([1] * 16, [3, 1, 7, 0, 5]):
+                seq, got = dec.open(), []
+                logits = dec.forward(seq, [5, 6, 7], [2])
+                for n in pieces:
+                    got += dec.decode_sampled(seq, logits, n, how)
+                    if n and len(got) < 16:
+                        logits = dec.forward(seq, got[-1:], [0])  # (the last one drawn has not been fed yet)
+                dec.close(seq)
+                assert got == want, pieces
