@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(PB_THREADS) pages_free_kernel(const __grid_con
       *entry = CUTB_NO_PAGE;
       if (p >= d.n_pages) {
         paged_report(d.status, CUTB_ERR_INVALID);
-      } else if (atomicSub(d.refs + p, 1u) == 0) {  // nobody held it
+      } else if (atomicSub(d.refs + p, 1u) - 1 >= 0x7fffffffu) {  // nobody held it (or others have just taken off as much: each of them puts its own back)
         atomicAdd(d.refs + p, 1u);
         paged_report(d.status, CUTB_ERR_INVALID);
       }

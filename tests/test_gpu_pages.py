@@ -221,3 +221,17 @@ def test_a_server_of_three_sequences():
     step([0, 1], [1, 20])
     step([2, 1, 0], [5, 1, 3])
     c.check()
+
+
+def test_tables_that_name_a_page_more_often_than_it_is_held():
+    """Freed at once, by many slots: the count ends at none, whatever order they come in, and the call reports it."""
+    from cut_b200 import _lib as L
+
+    for held in (0, 1, 3):
+        c, _ = pair(8, 400, 4)
+        c.tables[:, :2] = torch.tensor([5, 2], dtype=torch.int32)
+        c.lengths.fill_(20)
+        c.refs[5], c.refs[2] = held, 400
+        c.free(list(range(400)))
+        assert status(c) == L.ERR_INVALID
+        assert c.refs.tolist() == [0] * 8 and not c.lengths.any() and bool((c.tables == -1).all())
