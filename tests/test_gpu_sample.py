@@ -229,3 +229,58 @@ def test_two_threads_draw_from_rows_of_different_sizes():
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+def check_wide(x, u, t=None, k=None, p=None, least=None):
+    """As check(), the logarithms as near as many small weights allow: a weight is a whole number of units of 2^-42 of the largest, off by half
+    a unit (and what the exponential is off by, 2^-42 of the weight), so that the sum of n of them, which is at least 1, is off by n 2^-43
+    + 2^-42 of itself and the logarithm by as much."""
+    got, logs, st = run(x, u, t, k, p, least)
+    assert st == 0
+    rows, n = x.double().cpu().numpy(), len(u)
+    f = lambda v, d: np.full(n, d) if v is None else np.asarray(v, dtype=np.float32).astype(np.float64)  # noqa: E731
+    for r in range(n):
+        tok, lp = P.sampled(rows[r], f(t, 1)[r], 0 if k is None else k[r], f(p, 1)[r], f(least, 0)[r], float(np.float32(u[r])))
+        assert got[r] == tok, r
+        assert abs(logs[r] - lp) <= 2.0 ** -24 * abs(lp) + x.shape[1] * 2.0 ** -43 + 2.0 ** -36, (r, logs[r], lp)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("off", [0, 1])
+def test_rows_that_are_read_again_without_cut_offs(kind, off):
+    """So many rows that two blocks have one, and so wide that a block reads its part again instead of keeping it."""
+    r = np.random.default_rng(off)
+    n, vocab = 150, 128256
+    g = torch.Generator(device="cuda").manual_seed(off)
+    x = (2.5 * torch.randn(n, vocab + 3, device="cuda", generator=g)).to(TYPES[kind])[:, off: off + vocab - off]
+    u = r.random(n).astype(np.float32)
+    check_wide(x, u, t=r.choice([0.0, 0.5, 1.0, 2.0], n))
+    check_wide(x, u, t=r.choice([0.5, 1.0], n), least=r.choice([0.0, 0.01, 0.5, 1.0, 3.0], n))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [524288, 524287, 300001])
+def test_the_widest_rows(kind, vocab):
+    r = np.random.default_rng(vocab)
+    x = torch.from_numpy(r.choice([0.05, 2.5], (5, 1)) * r.standard_normal((5, vocab))).to(TYPES[kind]).cuda()
+    u = r.random(5).astype(np.float32)
+    check_wide(x, u)
+    check_wide(x, u, p=[0.9, 0.3, 0.999, 0.5, 0.95])
+    check_wide(x, u, k=[0, 3, 1000, 40, 260000], p=[0.9, 1.0, 0.99, 0.5, 0.95], least=[0, 0.01, 0, 0, 0.2])
+
+
+def test_the_widest_rows_whose_weights_fill_their_digits():
+    """All logits but one equal, with a weight whose lower two digits of 16 bits are as large as a search finds them: a block's 65536 of
+    them add up to just below 2^32 in either place."""
+    vocab = 524288
+    v = (1 + np.arange(1 << 22, dtype=np.float64) * 2.0 ** -23).astype(np.float32)
+    w = np.rint(np.exp(-v.astype(np.longdouble)) * np.longdouble(2.0) ** 42).astype(np.int64)
+    best = v[np.argmax(np.minimum(w & 0xffff, w >> 16 & 0xffff))]
+    weight = int(w[np.argmax(np.minimum(w & 0xffff, w >> 16 & 0xffff))])
+    assert min(weight & 0xffff, weight >> 16 & 0xffff) > 0xff00
+    x = torch.full((4, vocab), 0.0, device="cuda")
+    x[:] = -float(best)
+    for row, at in enumerate((0, 70001, 262144, vocab - 1)):
+        x[row, at] = 0.0
+    check_wide(x, [0.3333, 0.7777, 0.12345, 0.987], p=[0.5000123, 0.9000123, 0.2500123, 0.9990123])
+    check_wide(x, [0.3333, 0.7777, 0.12345, 0.987])
