@@ -542,6 +542,8 @@ def paged_desc(cache, n_tokens: int, dtype: torch.dtype, *, starts=None, slots=N
     """cutb_paged_desc of a call over `cache` (paged.PagedCache): sequence i is slot slots[i] (None: slot i), its rows are starts[i] ..
     starts[i + 1] - 1 of n_tokens (None: row i, one for each sequence).  max_new: at most so many rows of a sequence (None: as many as there are)."""
     _here("paged", cache.pages, cache.tables, cache.lengths, starts, slots, status)
+    if dtype not in _ELEMENTS or (max_new is not None and not 0 <= max_new < 1 << 32):
+        raise RuntimeError("paged: rows in float32, float16 or bfloat16, and a max_new that is not negative")
     d = L.PagedDesc()
     part = cache.layer_bytes() if layer or cache.pages.stride(0) != cache.pages.shape[1] else 0  # (whole pages: the call itself looks at layer 0)
     if layer < 0 or (layer + 1) * part > cache.pages.shape[1]:
@@ -612,6 +614,8 @@ def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=
     a sequence (1 without starts), and a bound near to them lets the call share its work out better."""
     hd = cache.head_dim
     _rows(q, n_heads, hd, "paged_attention: q")
+    if not 0 <= window < 1 << 32:
+        raise RuntimeError("paged_attention: a window of 0 (all keys) or more")
     _here("paged_attention", q, out, workspace)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -277,3 +277,17 @@ def test_rows_read_are_zero_where_nothing_is_read(monkeypatch):
     for kw in ({}, dict(slots=torch.tensor([9, 1, 2], dtype=torch.int32)), dict(starts=torch.tensor([0, 2], dtype=torch.int32))):
         k, v = ops.paged_kv_read(c, 3, dtype=torch.float32, **kw)
         assert k.shape == v.shape == (3, 64) and k.is_contiguous() and v.is_contiguous() and not k.any() and not v.any()
+
+
+def test_counts_below_zero_and_other_types_are_refused(monkeypatch):
+    """They would come to the call as counts of thousands of millions."""
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    c, q = PagedCache.allocate(4, 4, 200, 2, 32, page_tokens=16, device="cpu"), torch.zeros(2, 128)
+    for window in (-1, 1 << 32):
+        with pytest.raises(RuntimeError, match="window"):
+            ops.paged_attention(c, q, 4, window=window)
+    for max_new in (-1, 1 << 32):
+        with pytest.raises(RuntimeError, match="max_new"):
+            ops.paged_attention(c, q, 4, max_new=max_new)
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        ops.paged_kv_read(c, 2, dtype=torch.float64)
