@@ -543,3 +543,49 @@ def test_queries_that_are_not_finite_give_nan(kind, head, nh, kv, lengths, new):
                 ks, vs = kq[cut[s]: cut[s + 1], h * kv // nh], vq[cut[s]: cut[s + 1], h * kv // nh]
                 y, spread, products = P.attention(x[row, h], ks, vs, lengths[s] - new + row % new, scale, 0)
                 assert (np.abs(got[row, h] - y) <= P.tolerance(y, spread, products, scale, kind)).all(), (row, h)
+
+
+def repeated(c, tokens, kv, head, r):
+    """Fills pages 0, 1, .. of a cache whose table names them over and over, with positive values: what the cache holds of its
+    first `tokens` tokens, [kv, tokens, head] twice."""
+    from cut_b200 import ops
+
+    width = c.tables.shape[1]
+    c.tables.copy_((torch.arange(width, dtype=torch.int32) % (tokens // c.page_tokens)).expand_as(c.tables))
+    k, v = r.standard_normal((tokens, kv, head)).astype(np.float32), r.random((tokens, kv, head)).astype(np.float32)
+    c.lengths.fill_(tokens)
+    ops.paged_kv_write(c, cuda(k.reshape(tokens, -1)), cuda(v.reshape(tokens, -1)), starts=rows_of([tokens]), slots=rows_of([])[:1])
+    return P.quantised(k)[0].transpose(1, 0, 2), P.quantised(v)[0].transpose(1, 0, 2)
+
+
+def attention_repeated(q, k, v, pos, scale):
+    """P.attention over keys 0 .. pos that are k, v [tokens, head] over and over."""
+    n = len(k)
+    s = k @ q * scale
+    p = np.exp(s - s.max()) * ((pos + 1) // n + (np.arange(n) < (pos + 1) % n))
+    p /= p.sum()
+    return p @ v, p @ np.abs(v), float((np.abs(k) @ np.abs(q)).max())
+
+
+@pytest.mark.parametrize("kind,head,nh", [("f16", 64, 1), ("bf16", 64, 1), ("f32", 64, 1), ("f16", 128, 16), ("f16", 256, 2)])
+def test_single_rows_over_millions_of_keys(kind, head, nh):
+    """A hundred sequences of four million keys (the same pages over and over), so that a warp adds up hundreds of thousands of them:
+    values that are all positive, whose sum is large against each."""
+    from cut_b200 import ops
+    from cut_b200.paged import PagedCache
+
+    r = np.random.default_rng(head + nh)
+    n, base, length = 100, 4096, 4 << 20
+    c = PagedCache.allocate(base // 256, n, length, 1, head, page_tokens=256)
+    ks, vs = repeated(c, base, 1, head, r)
+    lengths = length - r.integers(0, 5000, n)
+    c.lengths.copy_(cuda(lengths.astype(np.int32)))
+    q = torch.from_numpy(0.1 * r.standard_normal((n, nh * head))).to(TYPES[kind]).cuda()
+    got, x, scale = ops.paged_attention(c, q, nh).double().cpu().numpy(), q.double().cpu().numpy(), float(np.float32(head ** -0.5))
+    c.check()
+    for s in range(n):
+        for h in range(nh):
+            part = slice(h * head, (h + 1) * head)
+            y, spread, products = attention_repeated(x[s, part], ks[0], vs[0], int(lengths[s]) - 1, scale)
+            off = np.abs(got[s, part] - y) - P.tolerance(y, spread, products, scale, kind)
+            assert off.max() <= 0, (s, h, off.max(), float(np.mean(got[s, part] / y - 1)))
