@@ -154,6 +154,7 @@ uint64_t paged_attention_workspace(const cutb_paged_desc &d);
 int paged_attention_launch(const cutb_paged_desc &d, cudaStream_t stream);
 // prompts, on the tensor cores (paged_prefill.cu); paged_attention_launch hands over
 bool paged_prefill_applies(const cutb_paged_desc &d);
+uint64_t paged_prefill_workspace(const cutb_paged_desc &d);
 int paged_prefill_launch(const cutb_paged_desc &d, cudaStream_t stream);
 int pages_reserve_launch(const cutb_pages_desc &d, cudaStream_t stream);
 int pages_fork_launch(const cutb_pages_desc &d, cudaStream_t stream);

@@ -562,7 +562,7 @@ template <typename T, int DP, int NT> int pt_launch(const cutb_paged_desc &d, co
 }  // namespace
 
 uint64_t paged_attention_workspace(const cutb_paged_desc &d) {
-  if (paged_prefill_applies(d)) return 0;
+  if (paged_prefill_applies(d)) return paged_prefill_workspace(d);
   PtPlan p;
   uint64_t bytes = 0;
   return pt_plan(d, &p, &bytes) == CUTB_OK ? bytes : 0;

@@ -34,9 +34,16 @@ template <typename T, int DP> struct PpShape {
   static constexpr uint32_t LOW = 128, OUT = 256, TOTAL = 384;
 };
 
+// Tensor cores cut a sum off at every product, by some 2^-22 of it: over 131072 keys the values of 16-bit rows came out 8.6e-4 too small, nearly
+// twice half a step of fp16.  So a sum goes on there for this many tiles (6e-5), and then is added to fp32 totals in the workspace, which calls
+// have that may see more keys.  fp32 rows are added up after every tile, in tensor memory; their sums and the weights' move to totals too (added one
+// by one, a million weights came out 2e-5 too small).  2048 rows behind 30720 keys in bf16: 1381 us, 1336 with one sum.
+constexpr uint32_t PP_SUM = 64;
+
 struct PpParams {
   float scale, sign;  // |scale| log2(e), and its sign (a scale of zero: queries of zero)
   uint32_t vec, out_vec;
+  float4 *totals;     // [block][DP / 4][row], where a row may see more than PP_SUM tiles
 };
 
 __device__ __forceinline__ float pp_exp2(float x) {
@@ -276,7 +283,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       const uint32_t desc_hi = (uint32_t)(proto >> 32), q_lo = (uint32_t)proto + ((q_u & 0x3FFFFu) >> 4), k_lo = (uint32_t)proto + ((k_u & 0x3FFFFu) >> 4);
       const uint32_t v_lo = (uint32_t)proto + ((v_u & 0x3FFFFu) >> 4);
       constexpr uint32_t id_s = umma_idesc_f16(128, 128), id_o = umma_idesc_f16(128, DP);
-      uint32_t sk = 0, pk = 0, sv = 0, pv = 0, pp_[2] = {0, 0}, acc[2] = {0, 0};
+      uint32_t sk = 0, pk = 0, sv = 0, pv = 0, pp_[2] = {0, 0}, acc[2] = {0, 0};  // acc: tiles in the sums
       bool ok = mbar_spin_bounded(qready, 0);
       tc_fence_after();
       auto scores = [&](uint32_t x) {
@@ -302,12 +309,12 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
 #pragma unroll
             for (uint32_t ks = 4 * half; ks < 4 * half + 4; ++ks)
               umma_ts(tmem + S::OUT + x * DP, tmem + (term + 1 < S::TERMS ? S::LOW : x * 128) + ks * 8, v_lo + sv * (VT >> 4) + (ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2, desc_hi, id_o,
-                      term | ks ? 1u : acc[x]);
+                      term | ks ? 1u : acc[x] != 0);
         }
         pp_[x] ^= 1u;
         umma_commit(odone + x * 8);
         if (last) umma_commit(vempty + sv * 8);
-        acc[x] = SPLIT ? 0 : 1;
+        if (!SPLIT) acc[x] = (acc[x] + 1) % PP_SUM;
         if (last && ++sv == SV) sv = 0, pv ^= 1u;
       };
       bool pending = false;  // the second row tile's value product over the tile before
@@ -420,8 +427,9 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
     }
     const float mult = mult_s[x * 128 + row];
     const uint32_t mine = tmem + ((warp & 3) << 21), s_t = mine + x * 128, l_t = mine + S::LOW, o_t = mine + S::OUT + x * DP, t_t = mine + S::TOTAL;
-    float low = -INFINITY, from = 0.f, l = 0.f;
+    float low = -INFINITY, from = 0.f, l = 0.f, low_sum = -INFINITY, l_sum = 0.f;  // low_sum: what the totals are relative to, l_sum: the weights'
     uint32_t ph = 0, done = 0;
+    float4 *totals = pp.totals + ((uint64_t)blockIdx.x * gridDim.y + kvh) * (ROWS * DP / 4) + x * 128 + row;  // (this thread's own, ROWS apart)
     bool dead = false;
     const uint32_t my_hi = hi[x], my_lo = lo[x], my_first = first_pos[x];
     for (uint32_t t = t_first; t < t_end; ++t) {
@@ -466,31 +474,53 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         f = low == to ? 1.f : pp_exp2(low - to);
         low = to, l *= f, from = to == -INFINITY ? 0.f : to;
       }
-      // The weighted values follow.  Those of fp32 rows leave the tensor cores after every tile and are added here: a sum that goes on
-      // there loses half a unit of its last place at every product of 16 keys.
-      if (done && (rises || SPLIT)) {
+      // The weighted values follow.  Those of fp32 rows leave the tensor cores after every tile and are added here, those of 16-bit rows after
+      // PP_SUM tiles.
+      const bool moves = done && done % PP_SUM == 0;  // the sums to the totals; the next tile begins anew
+      if (done && (rises || SPLIT || moves)) {
         if (!warp_wait(odone + x * 8, (done - 1) & 1u)) {
           dead = true;
           break;
         }
         tc_fence_after();
-#pragma unroll 1
-        for (uint32_t c = 0; c < DP; c += 16) {
-          uint32_t o[16];
+        auto sums = [&](uint32_t c, uint32_t (&o)[16]) {
           pp_ld16(o_t + c, o);
           if constexpr (SPLIT) {
-            if (done > 1) {
+            if ((done - 1) % PP_SUM) {
               uint32_t y[16];
               pp_ld16(t_t + c, y);
 #pragma unroll
               for (uint32_t i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(y[i]));
             }
           }
+        };
+        if (moves) {
+          const float ft = low_sum == low ? 1.f : pp_exp2(low_sum - low);
+#pragma unroll 2
+          for (uint32_t c = 0; c < DP; c += 16) {
+            float4 y[4] = {};
+            if (done > PP_SUM)
 #pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          tmem_st16(SPLIT ? t_t + c : o_t + c, o);
+              for (uint32_t i = 0; i < 4; ++i) y[i] = totals[(c / 4 + i) * ROWS];
+            uint32_t o[16];
+            sums(c, o);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+              totals[(c / 4 + i) * ROWS] = make_float4(fmaf(y[i].x, ft, __uint_as_float(o[4 * i]) * f), fmaf(y[i].y, ft, __uint_as_float(o[4 * i + 1]) * f),
+                                                       fmaf(y[i].z, ft, __uint_as_float(o[4 * i + 2]) * f), fmaf(y[i].w, ft, __uint_as_float(o[4 * i + 3]) * f));
+          }
+          l_sum = fmaf(l_sum, ft, l), l = 0.f, low_sum = low;
+        } else {
+#pragma unroll 1
+          for (uint32_t c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            sums(c, o);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(SPLIT ? t_t + c : o_t + c, o);
+          }
+          if constexpr (SPLIT) tmem_wait_st();
         }
-        if constexpr (SPLIT) tmem_wait_st();
       }
 #pragma unroll 1
       for (uint32_t j = 0; j < 4; ++j) {
@@ -529,6 +559,8 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
       if (lane == 0) give_up();
     } else if (done) {
       tc_fence_after();
+      const float ft = low_sum == low ? 1.f : pp_exp2(low_sum - low);
+      l = fmaf(l_sum, ft, l);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T *out = reinterpret_cast<T *>(d.out) + token * d.ldo + head;
 #pragma unroll 1
@@ -538,7 +570,7 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
         __syncwarp();
         pp_ld32(o_t + c, o);
         if constexpr (SPLIT) {
-          if (done > 1) {
+          if ((done - 1) % PP_SUM) {
             uint32_t y[32];
             pp_ld32(t_t + c, y);
 #pragma unroll
@@ -546,6 +578,14 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
           }
         }
         if (!live) continue;
+        if (done > PP_SUM) {
+#pragma unroll
+          for (uint32_t i = 0; i < 32; i += 4) {
+            const float4 y = totals[(c + i) / 4 * ROWS];
+            o[i] = __float_as_uint(fmaf(y.x, ft, __uint_as_float(o[i]))), o[i + 1] = __float_as_uint(fmaf(y.y, ft, __uint_as_float(o[i + 1])));
+            o[i + 2] = __float_as_uint(fmaf(y.z, ft, __uint_as_float(o[i + 2]))), o[i + 3] = __float_as_uint(fmaf(y.w, ft, __uint_as_float(o[i + 3])));
+          }
+        }
         if (pp.out_vec) {
           constexpr uint32_t N = 16 / sizeof(T);
 #pragma unroll
@@ -573,14 +613,16 @@ __global__ void __launch_bounds__(PpShape<T, DP>::WARPS * 32, 1) paged_prefill_k
   }
 }
 
+// a tile of rows for every 128 X of them, and one more for what each sequence leaves over
+uint64_t pp_row_tiles(const cutb_paged_desc &d, uint32_t X) { return (uint64_t)d.n_tokens * (d.n_heads / d.n_kv_heads) / (X * 128) + d.n_seqs; }
+
 template <typename T, int DP> int pp_launch(const cutb_paged_desc &d, cudaStream_t stream) {
   using S = PpShape<T, DP>;
   auto aligned = [&](const void *p, uint64_t ld) { return d.head_dim % 8 == 0 && ld * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   PpParams pp;
   pp.scale = d.scale == 0.f ? 1.f : fabsf(d.scale) * 1.4426950408889634f, pp.sign = d.scale == 0.f ? 0.f : d.scale < 0.f ? -1.f : 1.f;
-  pp.vec = aligned(d.q, d.ldq), pp.out_vec = aligned(d.out, d.ldo);
-  // a tile of rows for every 128 X of them, and one more for what each sequence leaves over
-  const uint64_t tiles = (uint64_t)d.n_tokens * (d.n_heads / d.n_kv_heads) / (S::X * 128) + d.n_seqs;
+  pp.vec = aligned(d.q, d.ldq), pp.out_vec = aligned(d.out, d.ldo), pp.totals = reinterpret_cast<float4 *>(d.workspace);
+  const uint64_t tiles = pp_row_tiles(d, S::X);
   CUTB_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
   CUTB_CUDA_TRY(launch_pdl(paged_prefill_kernel<T, DP>, dim3((uint32_t)tiles, d.n_kv_heads), dim3(S::WARPS * 32), S::SMEM, stream, d, pp));
   return CUTB_OK;
@@ -592,6 +634,17 @@ bool paged_prefill_applies(const cutb_paged_desc &d) {
   // (tensor memory does not hold the values of an fp32 tile of wider heads twice, beside its scores)
   if (d.dtype == CUTB_F32 && pg_pad(d.head_dim) > 128) return false;
   return (uint64_t)d.max_new * (d.n_heads / d.n_kv_heads) > 32;
+}
+
+// The totals of rows that may see more than PP_SUM tiles of keys: all the keys that a table holds, or a window's and those of the other
+// rows of a tile.
+uint64_t paged_prefill_workspace(const cutb_paged_desc &d) {
+  const uint32_t dp = pg_pad(d.head_dim);
+  uint64_t seen = (d.ld_table * d.page_tokens + PP_KEYS - 1) / PP_KEYS;
+  if (d.window) seen = min(seen, ((uint64_t)d.window + 126) / PP_KEYS + 2);
+  if (seen <= PP_SUM) return 0;
+  const uint32_t X = d.dtype == CUTB_F32 ? PpShape<float, 128>::X : dp > 128 ? PpShape<__half, 256>::X : PpShape<__half, 128>::X;
+  return pp_row_tiles(d, X) * d.n_kv_heads * X * 128 * dp * 4;
 }
 
 int paged_prefill_launch(const cutb_paged_desc &d, cudaStream_t stream) {

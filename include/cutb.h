@@ -737,8 +737,11 @@ CUTB_API int cutb_expert_down(const cutb_expert_desc *desc, void *stream);
  *                         (window 0: all of them); a row that sees none gives zeros, one of a query head that
  *                         is not finite NaN.  Query head h reads KV head h / (n_heads /
  *                         n_kv_heads).  Softmax and sums in fp32; fp32 queries and their weights enter the tensor cores as two fp16 terms,
- *                         16-bit ones as one.  `workspace`: cutb_paged_workspace_bytes(), 256-byte aligned, of no content before or after.
- *                         Calls that overlap need workspaces of their own.
+ *                         16-bit ones as one.  Weighted values are added up in fp32, at most 8192 keys' by the
+ *                         tensor cores alone (which lose up to 6e-5 of them).  `workspace`: cutb_paged_workspace_bytes(), 256-byte aligned,
+ *                         of no content before or after; prompts take one where a row may see more than 8192 keys (by the table's
+ *                         width and the window), 4 n_tokens n_heads head_dim bytes and a little more.  Calls that overlap need
+ *                         workspaces of their own.
  */
 enum { CUTB_NO_PAGE = 0xFFFFFFFFu }; /* an entry of a table behind a sequence's pages */
 typedef struct cutb_paged_desc {

@@ -589,3 +589,68 @@ def test_single_rows_over_millions_of_keys(kind, head, nh):
             y, spread, products = attention_repeated(x[s, part], ks[0], vs[0], int(lengths[s]) - 1, scale)
             off = np.abs(got[s, part] - y) - P.tolerance(y, spread, products, scale, kind)
             assert off.max() <= 0, (s, h, off.max(), float(np.mean(got[s, part] / y - 1)))
+
+
+@pytest.mark.parametrize("kind,head,nh,new,length,window", [("f16", 64, 1, 64, 1 << 20, 0), ("bf16", 64, 1, 64, 1 << 20, 0), ("f32", 64, 1, 64, 1 << 20, 0),
+                                                            ("f16", 128, 4, 100, 300000, 0), ("f16", 192, 4, 40, 280000, 0), ("f16", 256, 3, 50, 270000, 0),
+                                                            ("f16", 128, 2, 300, 400000, 262144), ("f16", 128, 1, 64, 8192 + 64, 0), ("f16", 40, 1, 200, 16500, 8300)])
+def test_prompts_behind_hundreds_of_thousands_of_keys(kind, head, nh, new, length, window):
+    """Prompts whose rows add up many thousands of positive values, and ones just past the keys that one sum goes on for."""
+    from cut_b200 import ops
+    from cut_b200.paged import PagedCache
+
+    r = np.random.default_rng(head + new)
+    base = 2048
+    c = PagedCache.allocate(base // 64, 3, length + 100, 1, head, page_tokens=64)
+    ks, vs = repeated(c, base, 1, head, r)
+    lengths, rows = [length, 1000, length - 3000], [new, 100, new // 2 + 33]  # (and a short one between them)
+    c.lengths.copy_(cuda(np.array(lengths, dtype=np.int32)))
+    n = sum(rows)
+    q = torch.from_numpy(0.1 * r.standard_normal((n, nh * head))).to(TYPES[kind]).cuda()
+    out = ops.paged_attention(c, q, nh, starts=rows_of(rows), max_new=max(rows), window=window)
+    again = ops.paged_attention(c, q, nh, starts=rows_of(rows), max_new=max(rows), window=window)
+    c.check()
+    assert torch.equal(out, again)
+    got, x, scale, row = out.double().cpu().numpy(), q.double().cpu().numpy(), float(np.float32(head ** -0.5)), 0
+    for s, m in enumerate(rows):
+        for i in range(m):
+            pos = lengths[s] - m + i
+            if i % 9 and i + 1 < m:
+                row += 1
+                continue
+            for h in range(nh):
+                part = slice(h * head, (h + 1) * head)
+                if window and pos >= window:  # the keys from pos + 1 - window on
+                    at = (pos + 1 - window) % base
+                    y, spread, products = attention_repeated(x[row, part], np.roll(ks[0], -at, 0), np.roll(vs[0], -at, 0), window - 1, scale)
+                else:
+                    y, spread, products = attention_repeated(x[row, part], ks[0], vs[0], pos, scale)
+                off = np.abs(got[row, part] - y) - P.tolerance(y, spread, products, scale, kind)
+                assert off.max() <= 0, (s, i, h, off.max(), float(np.mean(got[row, part] / y - 1)))
+            row += 1
+
+
+def test_scores_that_rise_over_many_keys():
+    """The reference of the weights moves while sums are on their way to the totals, and stays where rows have seen their largest early."""
+    from cut_b200 import ops
+    from cut_b200.paged import PagedCache
+
+    r = np.random.default_rng(13)
+    n, head, rows = 40000, 64, 130
+    c = PagedCache.allocate(n // 64, 1, n, 1, head, page_tokens=64)
+    c.tables[0] = torch.arange(n // 64, dtype=torch.int32)
+    c.lengths.fill_(n)
+    direction = r.standard_normal(head)
+    k = (np.linspace(-40, 40, n)[:, None] * direction / head + 0.02 * r.standard_normal((n, head))).astype(np.float32)
+    v = r.standard_normal((n, head)).astype(np.float32)
+    ops.paged_kv_write(c, cuda(k), cuda(v), starts=rows_of([n]))
+    kq, vq = P.quantised(k)[0], P.quantised(v)[0]
+    q = np.tile(direction, (rows, 2)) * r.choice([-1.0, 0.02, 1.0, 0.3], (rows, 1))
+    for kind in ("f16", "bf16"):
+        x = torch.from_numpy(q).to(TYPES[kind]).cuda()
+        got = ops.paged_attention(c, x, 2, starts=rows_of([rows]), max_new=rows, scale=1.0).double().cpu().numpy()
+        x = x.double().cpu().numpy()
+        for i in range(0, rows, 7):
+            y, spread, products = P.attention(x[i, :head], kq, vq, n - rows + i, 1.0, 0)
+            assert (np.abs(got[i, :head] - y) <= P.tolerance(y, spread, products, 1.0, kind)).all(), (kind, i)
+    c.check()

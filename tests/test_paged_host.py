@@ -291,3 +291,15 @@ def test_counts_below_zero_and_other_types_are_refused(monkeypatch):
             ops.paged_attention(c, q, 4, max_new=max_new)
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
         ops.paged_kv_read(c, 2, dtype=torch.float64)
+
+
+def test_scratch_of_prompts_behind_many_keys():
+    """Rows that may see more than 8192 keys have their sums moved to totals in the scratch, 4 bytes an element of whole tiles of rows."""
+    need = lambda **kw: L.lib().cutb_paged_workspace_bytes(C.byref(desc(**{**dict(n_seqs=1, n_tokens=1000, max_new=1000, starts=256), **kw})))  # noqa: E731
+    tiles = {L.F16: 1000 * 4 // 256 + 1, L.F32: 1000 * 4 // 128 + 1}
+    for kind, rows in ((L.F16, 256), (L.F32, 128)):
+        assert need(dtype=kind, ld_table=128) == 0  # 8192 keys
+        assert need(dtype=kind, ld_table=129) == tiles[kind] * 8 * rows * 128 * 4
+        assert need(dtype=kind, ld_table=9999, window=62 * 128 + 1) == 0 and need(dtype=kind, ld_table=9999, window=8192) > 0
+        refused("cutb_paged_attention", desc(n_seqs=1, n_tokens=1000, max_new=1000, starts=256, dtype=kind, ld_table=129), "workspace", L.ERR_WORKSPACE)
+    assert need(dtype=L.BF16, ld_table=129, n_kv_heads=2, n_heads=6, head_dim=200, ldq=1200, ldo=1200) == (1000 * 3 // 128 + 1) * 2 * 128 * 256 * 4
