@@ -554,13 +554,15 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) paged_kv_
   if (!sq.bad && row - sq.row0 >= sq.rows) return;
   const uint32_t pos = sq.len - sq.rows + (row - sq.row0);
   const uint32_t page = sq.bad ? CUTB_NO_PAGE : d.tables[sq.slot * d.ld_table + pos / d.page_tokens];
-  if (page >= d.n_pages) {
-    if (lane == 0) paged_report(d.status, CUTB_ERR_INVALID);
-    return;
-  }
   const bool value = h >= d.n_kv_heads;
   const uint32_t kvh = value ? h - d.n_kv_heads : h;
   T *dst = reinterpret_cast<T *>(value ? d.v_out : d.k_out) + row * (value ? d.ldv_out : d.ldk_out) + (uint64_t)kvh * d.head_dim;
+  if (page >= d.n_pages) {
+    if (lane == 0) paged_report(d.status, CUTB_ERR_INVALID);
+    if (!d.starts)  // (the row is this sequence's whatever else is wrong: callers need not fill the rows first)
+      for (uint32_t i = lane; i < d.head_dim; i += 32) dst[i] = from_f<T>(0.f);
+    return;
+  }
   const Unit u = unit_of(d, page, kvh, pos, value);
   for (uint32_t i = 4 * lane; i < d.head_dim; i += 128) {
     float x[4];
@@ -627,8 +629,8 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_
   });
 }
 
-// By units where their warps are sixteen to an SM and sequences have units; else a warp per head of a row.
-bool by_units(const cutb_paged_desc &d, uint64_t heads) { return d.max_new >= PG_UNIT && (d.n_tokens + PG_UNIT - 1) / PG_UNIT * heads >= 148 * 16; }
+// By units where their warps are sixteen to an SM and sequences may have units (without starts they have a row each); else a warp per head of a row.
+bool by_units(const cutb_paged_desc &d, uint64_t heads) { return d.starts && d.max_new >= PG_UNIT && (d.n_tokens + PG_UNIT - 1) / PG_UNIT * heads >= 148 * 16; }
 uint32_t units_of(const cutb_paged_desc &d) { return (d.n_tokens + PG_UNIT - 1) / PG_UNIT; }
 dim3 warps_grid(uint64_t warps) { return dim3((uint32_t)((warps + 7) / 8)); }
 

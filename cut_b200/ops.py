@@ -600,7 +600,11 @@ def paged_kv_read(cache, n_tokens: int, *, dtype: torch.dtype = torch.float16, s
                   status=None):
     """(keys, values) [n_tokens, n_kv_heads * head_dim] that the sequences' last rows stand for in the cache; rows that no sequence has,
     and those of sequences, tables and pages that the call reports, are zero."""
-    k, v = cache.pages.new_zeros((2, n_tokens, cache.n_kv_heads * cache.head_dim), dtype=dtype)  # (one fill)
+    shape = (n_tokens, cache.n_kv_heads * cache.head_dim)
+    if starts is None:  # (every row is written)
+        k, v = cache.pages.new_empty(shape, dtype=dtype), cache.pages.new_empty(shape, dtype=dtype)
+    else:
+        k, v = cache.pages.new_zeros((2, *shape), dtype=dtype)  # (one fill)
     d = paged_desc(cache, n_tokens, dtype, starts=starts, slots=slots, max_new=max_new, layer=layer, status=status)
     d.k_out, d.ldk_out, d.v_out, d.ldv_out = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
     L.check(L.lib().cutb_paged_kv_read(C.byref(d), _stream_ptr()))

@@ -732,7 +732,8 @@ CUTB_API int cutb_expert_down(const cutb_expert_desc *desc, void *stream);
  *                         Turned: the first rot_dims elements of a head, tables [max_pos][rot_dims / 2], rot_pairing as in
  *                         cutb_window_attn_desc; products and sums are rounded separately in fp32.  max_pos is only looked at with
  *                         rot_dims.  No slot may be named twice, and q_out shares no memory with q, k and v.
- *   cutb_paged_kv_read    k_out, v_out = the values that the sequences' last rows stand for in the cache
+ *   cutb_paged_kv_read    k_out, v_out = the values that the sequences' last rows stand for in the cache; without starts, zeros for
+ *                         the row of a sequence that is reported
  *   cutb_paged_attention  out = attention of the (turned) queries: a row at position p sees the keys j <= p with p - j < window
  *                         (window 0: all of them); a row that sees none gives zeros, one of a query head that
  *                         is not finite NaN.  Query head h reads KV head h / (n_heads /

@@ -654,3 +654,31 @@ def test_scores_that_rise_over_many_keys():
             y, spread, products = P.attention(x[i, :head], kq, vq, n - rows + i, 1.0, 0)
             assert (np.abs(got[i, :head] - y) <= P.tolerance(y, spread, products, 1.0, kind)).all(), (kind, i)
     c.check()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("head,kv,n,max_new", [(64, 2, 6, None), (33, 3, 6, None), (128, 32, 900, 16)])
+def test_every_row_that_is_read_without_starts_is_written(kind, head, kv, n, max_new):
+    """Few rows, and as many as whole units would be read by: the rows of sequences that cannot be read are zero, whatever was there."""
+    import ctypes as C
+
+    from cut_b200 import _lib as L
+    from cut_b200 import ops
+
+    r = np.random.default_rng(14)
+    lengths = [20, 33, 0, 7]
+    c = make_cache(lengths, kv, head, 16, r)
+    ks, vs = fill_cache(c, lengths, kv, head, r)
+    c.tables[3, 0], slots = 1 << 20, r.choice([0, 1, 2, 3, 77, -1], n).astype(np.int32)
+    slots[:3] = 2, 0, 77
+    k, v = (torch.full((n, kv * head), 7.0, dtype=TYPES[kind], device="cuda") for _ in range(2))
+    sl = cuda(slots)
+    d = ops.paged_desc(c, n, TYPES[kind], slots=sl, max_new=max_new)
+    d.k_out, d.ldk_out, d.v_out, d.ldv_out = k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0)
+    L.check(L.lib().cutb_paged_kv_read(C.byref(d), ops._stream_ptr()))
+    with pytest.raises(L.CutbError) as e:
+        c.check()
+    assert e.value.status == L.ERR_INVALID
+    for got, held in ((k, ks), (v, vs)):
+        want = np.stack([held[s][:, -1].reshape(-1) if s in (0, 1) else np.zeros(kv * head) for s in slots])
+        assert torch.equal(got.cpu(), torch.from_numpy(want).to(TYPES[kind]))
