@@ -6,13 +6,15 @@
 // 16-bit rows take 8 columns.  fp32 rows enter as two fp16 terms: a tile of 8 columns has the high parts of four rows and then their low
 // parts, and so have the weights (22 bits of each; the products are exact, the sums fp32).  Queries are scaled by a power of two so
 // that the largest element is in [1, 2), weights are kept between 2^8
-// and 2^15 at their largest: fp16 holds 2^-24 of the former and 2^-32 of the largest weight.
+// and 2^15 at their largest: fp16 holds 2^-24 of the former and 2^-32 of the largest weight.  The weights of 16-bit rows enter as one fp16 number,
+// 11 bits: bf16 outputs are as far from the exact ones as rounding takes them, fp16 ones 2.7e-4 instead of 2.1e-4 (over 131072 keys); a second
+// term would double the products of the values.
 //
-// Bound by HBM: 2560 bytes of a 128-element unit are 4096 elements, and about 290 warp instructions.  Units are copied whole by bulk
+// A unit of 128-element heads is 2560 bytes and about 290 warp instructions.  Units are copied whole by bulk
 // copies, each warp through a ring of its own, so that a block has up to 80 KB in flight and warps meet only at the ends.
 // 64 sequences of 3000 tokens, 32 heads of 128 over 8 KV heads, in bf16: 68 us, 3.6 TB/s; of 8000 in fp32: 147 us, 4.4 TB/s; 2 of 131072 in
-// fp16: 81 us, 4.2 TB/s.  Four warps to a scheduler (their registers hold the values' sums) issue in 58 % of the cycles, most of it
-// nibbles becoming fp16; a token of 1500 takes 14 us, two launches' latencies.
+// fp16: 82 us, 4.1 TB/s.  What holds it back is that only four warps fit a scheduler (127 registers: the values' sums are in them), which issue in 57 %
+// of the cycles, most of it nibbles becoming fp16; a token of 1500 takes 14 us, two launches' latencies.
 // Two units a step: what a step costs besides its products (the copy, the maximum over the lanes) is paid half as often.
 // The steps of all sequences and KV heads in a row are shared out evenly over the blocks.  Where a block's part begins or ends inside
 // a KV head's units, its maxima, sums and values go to the workspace, and a second kernel joins them in their order.
@@ -33,7 +35,7 @@ struct PtSeq {
 __device__ __forceinline__ uint64_t pt_div(uint64_t a, uint64_t b) {  // (a 64-bit division takes some hundred cycles)
   return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
 }
-// The shares of the blocks: `each` steps, the first `more` of them one more; at least PT_WARPS steps in each.
+// The shares of the blocks: `each` steps, the first `more` of them one more; a block for every PT_WARPS steps at most.
 struct PtShares {
   uint64_t each, more;
   uint32_t n;

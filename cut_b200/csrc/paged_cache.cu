@@ -438,8 +438,8 @@ template <typename T, bool VEC> __device__ __forceinline__ void turn_row(const c
 }
 
 // A warp per head of a piece: a whole unit is put together in shared memory, four tokens at a time, and stored in 16-byte pieces; the warps
-// behind those turn the queries.  13426 rows of 32 + 2 * 8 heads of 128 in bf16: 92 us, 50 without queries, where reading them takes 9 (some 2000
-// instructions a unit, most of them in the ALU; four blocks to an SM: with two and more rows on their way at a time 70 us).  A warp per head
+// behind those turn the queries.  13426 rows of 32 + 2 * 8 heads of 128 in bf16: 94 us, 50 without queries, where reading them takes 9: loads
+// that nothing covers are the longest wait (7.8 cycles an instruction, 52 % of the issue slots used; some 2000 instructions a unit).  A warp per head
 // of a row, bytes stored one by one, took 400 with the reading.
 template <typename T, bool VEC> __global__ void __launch_bounds__(256, 4) paged_kv_write_units_kernel(const __grid_constant__ cutb_paged_desc d) {
   __shared__ __align__(16) uint8_t stage_s[8][PC_STAGE];

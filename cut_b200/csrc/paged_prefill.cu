@@ -12,8 +12,11 @@
 //                   its units keep four neighbouring tokens together; 128-byte swizzle.
 // A tile of 128 keys costs 256 rows of 128 elements about 2000 cycles of tensor cores, as many of exponentials, and the unpacking 800
 // issue slots a scheduler, which run beside one another: two row tiles alternate, and the weights of 64 keys at a time are handed over.
-// 8192 tokens of 32 heads (8 KV heads) of 128 in bf16: 693 us, 793 TFLOP/s of the half that is seen; 4 x 1500 behind 1500 more: 356 us; 512
-// tokens in fp32: 25 us, of which one tile's chain of products, exponentials and products is the most.
+// 8192 tokens of 32 heads (8 KV heads) of 128 in bf16: 703 us, 782 TFLOP/s of the half that is seen; 4 x 1500 behind 1500 more: 362 us; 512
+// tokens in fp32: 26 us, of which one tile's chain of products, exponentials and products is the most.
+// Weights of 16-bit rows are one fp16 number, as in the kernel for few rows.
+// The keys of a row tile are one block's work however many they are: a few rows behind a long cache that come here (more than 32 query rows of a
+// KV head) leave most SMs idle, 5 rows of 64 heads behind 100000 keys 1803 us, 4 rows, by the other kernel, 89.
 // Every wait is bounded; on expiry the block records CUTB_ERR_TIMEOUT, frees its tensor memory and returns (it has no copies in flight).
 #include "kernels.h"
 #include "paged_common.cuh"

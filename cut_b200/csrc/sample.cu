@@ -9,7 +9,7 @@
 // are compared with one another, or where they are many found by their keys, 11 bits at a time.  A top-k up to 256 needs a histogram of
 // the threads' largest logits only.  Equal logits are cut off by their index.  The draw adds up the kept weights in the order of the indices.
 // Bound by instructions and, for few rows, by barriers: 1 x 32000 fp32 logits with every cut-off 10 us, 64 of them 14 (with top-p alone
-// 31), 256 x 128256 bf16 logits without cut-offs 68 us, with top-k and top-p 44, with top-p alone 277.
+// 33), 256 x 128256 bf16 logits without cut-offs 68 us, with top-k and top-p 48, with top-p alone 291.
 #include <cooperative_groups.h>
 
 #include <type_traits>

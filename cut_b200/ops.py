@@ -569,7 +569,8 @@ def paged_kv_write(cache, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor |
                    slots=None, max_new: int | None = None, cos_t=None, sin_t=None, rot_dims: int = 0, pairing: int = L.ROT_HALVES, layer: int = 0,
                    status=None):
     """Stores the rows k, v [n, n_kv_heads * head_dim] of the sequences' last tokens (cache.lengths counts them already), keys turned at
-    their positions, in 4 bits; with q [n, n_heads * head_dim] returns the turned queries."""
+    their positions, in 4 bits; with q [n, n_heads * head_dim] returns the turned queries (rows that no sequence has are not written:
+    in q_out as they were, in a new tensor undefined)."""
     hk, hd = cache.n_kv_heads, cache.head_dim
     _rows(k, hk, hd, "paged_kv_write: k"), _rows(v, hk, hd, "paged_kv_write: v")
     if v.dtype != k.dtype or v.shape[0] != k.shape[0] or (q is not None and (q.dtype != k.dtype or q.shape[0] != k.shape[0])):
@@ -614,8 +615,11 @@ def paged_kv_read(cache, n_tokens: int, *, dtype: torch.dtype = torch.float16, s
 def paged_attention(cache, q: torch.Tensor, n_heads: int, *, starts=None, slots=None, max_new: int | None = None, window: int = 0,
                     scale: float | None = None, layer: int = 0, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                     status=None) -> torch.Tensor:
-    """Attention of the turned queries q [n, n_heads * head_dim] of the sequences' last tokens over the cache; max_new bounds the rows of
-    a sequence (1 without starts), and a bound near to them lets the call share its work out better."""
+    """Attention of the turned queries q [n, n_heads * head_dim] of the sequences' last tokens over the cache.  max_new bounds the rows of
+    a sequence (None: 1 without starts, with them all n), and one near to them matters: up to 32 query rows of a KV head (max_new times
+    n_heads / n_kv_heads) the keys of a sequence are shared out over the GPU, above that a block walks them for every 128 or 256 rows.
+    Rows that no sequence has are not written: in `out` as they were, in a new tensor undefined.  workspace: scratch to use instead of a
+    new one (paged_workspace(); prompts take some where a table holds more than 8192 keys)."""
     hd = cache.head_dim
     _rows(q, n_heads, hd, "paged_attention: q")
     if not 0 <= window < 1 << 32:

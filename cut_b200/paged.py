@@ -8,8 +8,9 @@
     cache.free(slots)                     the sequences end
     cache.compact()                       the pages in use move to the pool's beginning
 
-Every call runs on the current stream and reads its slots and counts from device memory (lists are copied there first); none waits
-for the device.  What a call finds wrong on the device is in `status`, which check() reads."""
+Every call runs on the current stream and reads its slots and counts from device memory: int32 tensors there, which a recorded
+call reads anew, or lists, which are copied first (the copy waits for the stream, and cannot be recorded).  With tensors no call waits for
+the device.  What a call finds wrong on the device is in `status`, which check() reads."""
 from __future__ import annotations
 
 import ctypes as C
@@ -112,7 +113,7 @@ class PagedCache:
         self._run("cutb_pages_compact", self._desc(), True)
 
     def copy(self, src, dst) -> None:
-        """Page dst[i] becomes a copy of page src[i] (tables and refs are the caller's)."""
+        """Page dst[i] becomes a copy of page src[i], every dst named once (tables and refs are the caller's)."""
         self._whole("copy")
         src = self._vector(src)
         dst = self._vector(dst, src.numel())

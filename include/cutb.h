@@ -785,7 +785,7 @@ CUTB_API int cutb_paged_attention(const cutb_paged_desc *desc, void *stream);
  *   cutb_pages_free     slot items[i] is empty, its pages held once less; freeing an empty slot changes nothing
  *   cutb_pages_compact  moves the pages that are held to the places 0, 1, ..: those past the count of held pages, in their order, to
  *                       the free places below it; tables and refs follow
- *   cutb_pages_copy     page others[i] = page items[i]; no page may be both
+ *   cutb_pages_copy     page others[i] = page items[i]; no page may be both, and none named twice among the others
  * workspace: cutb_pages_workspace_bytes(), 256-byte aligned, of no content before or after (fork, free and copies need none).
  */
 typedef struct cutb_pages_desc {
@@ -813,8 +813,8 @@ CUTB_API int cutb_pages_copy(const cutb_pages_desc *desc, void *stream);
  *   least one), of those the ones with w_i >= min_p (at least one, the first); the token is the first kept i, by index, whose sum of weights up to
  *   and with it is above u times the sum of all kept ones.  temperature 0: the largest logit.
  * temperature, top_k, top_p, min_p: a value per row in device memory; null: 1, 0, 1, 0.  logprobs (optional): the logarithm of the
- * token's share of the kept weight.  Weights are sums of 2^-42 of the largest, exactly added: the order of the additions is of no
- * account.  A NaN counts as minus infinity; if the largest is plus infinity, its places share the weight.  A row with no
+ * token's share of the kept weight.  Weights are whole numbers of 2^-42 of the largest, exactly added: the order of the additions is of no
+ * account, a token below half of that is not drawn, and the logarithm is within vocab 2^-43 of the exact one, and rounded.  A NaN counts as minus infinity; if the largest is plus infinity, its places share the weight.  A row with no
  * logit above minus infinity gives CUTB_NO_TOKEN and minus infinity.  A temperature that is negative or not finite, a NaN among the settings or
  * a u outside [0, 1) gives the same and sets *status to CUTB_ERR_INVALID.
  */
