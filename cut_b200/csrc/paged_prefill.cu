@@ -40,7 +40,7 @@ template <typename T, int DP> struct PpShape {
 // Tensor cores cut a sum off at every product, by some 2^-22 of it: over 131072 keys the values of 16-bit rows came out 8.6e-4 too small, nearly
 // twice half a step of fp16.  So a sum goes on there for this many tiles (6e-5), and then is added to fp32 totals in the workspace, which calls
 // have that may see more keys.  fp32 rows are added up after every tile, in tensor memory; their sums and the weights' move to totals too (added one
-// by one, a million weights came out 2e-5 too small).  2048 rows behind 30720 keys in bf16: 1381 us, 1336 with one sum.
+// by one, a million weights came out 2e-5 too small).  The last 2048 rows of 32768 in bf16: 1381 us, 1336 with one sum.
 constexpr uint32_t PP_SUM = 64;
 
 struct PpParams {
